@@ -24,6 +24,7 @@
 #define HS_STATUS_BAD_POSITION 2
 #define HS_STATUS_BAD_PAGE 4
 #define HS_STATUS_PIPELINE_TIMEOUT 8
+#define HS_STATUS_BAD_ROW 16             // a record or mask outside its table
 
 #define HS_DT_F32 0
 #define HS_DT_BF16 1

@@ -1,0 +1,87 @@
+// Copies of cache pages, in every cache entry of a group at once.
+//
+// A pool is [entries, pages, tiles, rows, row bytes] (tiles: planes x heads).  For each listed pair
+// i and each entry e:  dst[e, d_i, :, :r_i] = src[e, s_i, :, :r_i];  rows behind the first r_i of a
+// page stay as they were.  dst and src may be one pool: the caller sees to it that no page is
+// written twice, nor written and read.  The list travels as a kernel argument, so that no copy of
+// it has to be made on the device, and kept there, before the launch.
+#include "common.cuh"
+
+namespace hs {
+
+constexpr int PC_THREADS = 256, PC_PAIRS = 1024;
+
+struct PageList {
+  int dst[PC_PAIRS], src[PC_PAIRS];
+  short rows[PC_PAIRS];
+};
+
+template <typename V>
+__global__ void __launch_bounds__(PC_THREADS)
+copy_pages_kernel(V* dst, const V* src, long long dst_pages, long long src_pages, int tiles,
+                  int page_rows, int row_vecs, const __grid_constant__ PageList list) {
+  pdl_trigger();
+  pdl_wait();
+  const int i = blockIdx.x, e = blockIdx.y;
+  const int rows = list.rows[i];
+  const int tile_vecs = page_rows * row_vecs, live = rows * row_vecs;
+  const size_t page_vecs = (size_t)tiles * tile_vecs;
+  V* to = dst + (e * dst_pages + list.dst[i]) * page_vecs;
+  const V* from = src + (e * src_pages + list.src[i]) * page_vecs;
+  for (int j = threadIdx.x; j < tiles * live; j += PC_THREADS) {
+    const int at = j / live * tile_vecs + j % live;
+    to[at] = from[at];
+  }
+}
+
+template <typename V>
+cudaError_t copy_pages(void* dst, const void* src, int n, const int* dst_list, const int* src_list,
+                       const int* rows, int entries, int dst_pages, int src_pages, int tiles,
+                       int page_rows, int row_bytes, cudaStream_t stream) {
+  for (int from = 0; from < n; from += PC_PAIRS) {
+    const int count = n - from < PC_PAIRS ? n - from : PC_PAIRS;
+    PageList list;
+    for (int i = 0; i < count; ++i) {
+      list.dst[i] = dst_list[from + i];
+      list.src[i] = src_list[from + i];
+      list.rows[i] = (short)(rows ? rows[from + i] : page_rows);
+    }
+    const cudaError_t e = hs_launch(copy_pages_kernel<V>, dim3(count, entries), dim3(PC_THREADS), 0,
+                                    stream, hs_pdl_enabled(), (V*)dst, (const V*)src,
+                                    (long long)dst_pages, (long long)src_pages, tiles, page_rows,
+                                    (int)(row_bytes / sizeof(V)), list);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace hs
+
+// The lists (n numbers each; rows may be null: whole pages) are in host memory and are read before
+// this returns.  Numbers outside the pools are refused here, before anything is launched.
+HS_EXPORT int hs_copy_pages(void* dst, const void* src, int n, const int* dst_list,
+                            const int* src_list, const int* rows, int entries, int dst_pages,
+                            int src_pages, int tiles, int page_rows, int row_bytes, void* stream) {
+  if (n <= 0) return HS_OK;
+  if (!dst || !src || !dst_list || !src_list) return HS_ERR_ARGUMENT;
+  if (entries <= 0 || entries > 65535 || tiles <= 0 || page_rows <= 0 || page_rows > 32767 ||
+      row_bytes <= 0 || row_bytes % 2 || (long long)tiles * page_rows * row_bytes > 0x7fffffffLL)
+    return HS_ERR_UNSUPPORTED;
+  for (int i = 0; i < n; ++i)
+    if (dst_list[i] < 0 || dst_list[i] >= dst_pages || src_list[i] < 0 || src_list[i] >= src_pages ||
+        (rows && (rows[i] < 0 || rows[i] > page_rows)))
+      return HS_ERR_ARGUMENT;
+  const uintptr_t bits = (uintptr_t)dst | (uintptr_t)src | (uintptr_t)row_bytes;
+  cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t e;
+  if (bits % 16 == 0)
+    e = hs::copy_pages<uint4>(dst, src, n, dst_list, src_list, rows, entries, dst_pages, src_pages,
+                              tiles, page_rows, row_bytes, st);
+  else if (bits % 4 == 0)
+    e = hs::copy_pages<uint32_t>(dst, src, n, dst_list, src_list, rows, entries, dst_pages, src_pages,
+                                 tiles, page_rows, row_bytes, st);
+  else
+    e = hs::copy_pages<uint16_t>(dst, src, n, dst_list, src_list, rows, entries, dst_pages, src_pages,
+                                 tiles, page_rows, row_bytes, st);
+  return e == cudaSuccess ? HS_OK : (int)e;
+}

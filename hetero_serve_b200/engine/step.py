@@ -32,7 +32,8 @@ from ..cache import CacheManager, CacheStorage, GroupSpec, OutOfPages
 from ..kernels.ops import size_class
 
 STATUS_BITS = {1: "a token id outside the vocabulary", 2: "a position outside the table",
-               4: "a page number outside the pool", 8: "a kernel pipeline timed out"}
+               4: "a page number outside the pool", 8: "a kernel pipeline timed out",
+               16: "a token record or grammar mask outside its table"}
 
 
 class StepError(RuntimeError):

@@ -1,3 +1,4 @@
-from .ops import AttentionGeometry, AttentionPlan, CudaOps, KernelError, load_library
+from .ops import AttentionGeometry, AttentionPlan, CudaOps, KernelError, TokenHistory, load_library
 
-__all__ = ["AttentionGeometry", "AttentionPlan", "CudaOps", "KernelError", "load_library"]
+__all__ = ["AttentionGeometry", "AttentionPlan", "CudaOps", "KernelError", "TokenHistory",
+           "load_library"]

@@ -17,6 +17,7 @@ import math
 from ctypes import c_float, c_int, c_void_p
 from dataclasses import dataclass
 
+import numpy as np
 import torch
 
 from . import build as _build
@@ -133,6 +134,32 @@ class FusedTables:
         return self.data.data_ptr() + self.n_layers * self.layer_bytes
 
 
+@dataclass
+class TokenHistory:
+    """Which tokens the request in each state slot holds, in device memory: what penalties for
+    repeated tokens go by.  ``prompt`` and ``output`` are bits over the vocabulary (bit v % 32
+    of word v // 32: v stands in the prompt; v has been generated), ``counts`` says how often v
+    has been generated and is read only where its output bit is set."""
+
+    prompt: torch.Tensor          # [slots, words] int32
+    output: torch.Tensor          # [slots, words] int32
+    counts: torch.Tensor          # [slots, vocab] int32
+
+    @classmethod
+    def zeros(cls, slots: int, vocab: int, device) -> "TokenHistory":
+        z = lambda n: torch.zeros(slots, n, dtype=torch.int32, device=device)     # noqa: E731
+        return cls(z(history_words(vocab)), z(history_words(vocab)), z(vocab))
+
+    def tensors(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        return self.prompt, self.output, self.counts
+
+
+def history_words(vocab: int) -> int:
+    """Words of 32 bits that hold a bit per token of the vocabulary."""
+    return -(-vocab // 32)
+
+
+MAX_ALTERNATIVES = 32     # most alternatives a row of ``token_logprobs`` can have
 DECODE_MAX_NEW = 4        # requests bringing at most this many tokens use the decode kernel
 PREFILL_TILE = 128
 
@@ -164,6 +191,48 @@ def plan_decode_ints(n_rows: int) -> int:
     """Ints of the single-query section: 3 per token, padded so that the tile section that
     follows is 16-byte aligned."""
     return (3 * n_rows + 3) // 4 * 4
+
+
+PAGE_LIST = 1024          # pages a launch of the page copy takes
+
+
+def page_lists(dst_pages, src_pages, rows, n_dst, n_src, page_rows, one_pool):
+    """The lists of a page copy as int32 arrays (``rows`` may be None).  Refused are lists of
+    different lengths or of anything but whole numbers, that reach outside their pools, write a
+    page twice, or, inside one pool, write a page that is also read."""
+    out = []
+    for nm, given, least, most in (("written", dst_pages, 0, n_dst - 1),
+                                   ("read", src_pages, 0, n_src - 1),
+                                   ("filled rows", rows, 0, page_rows)):
+        if given is None:
+            out.append(None)
+            continue
+        a = np.asarray(given)
+        if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
+            raise KernelError(f"copy_pages: {nm}: a list of whole numbers wanted")
+        if a.size and (int(a.min()) < least or int(a.max()) > most):
+            raise KernelError(f"copy_pages: {nm}: a number lies outside [{least}, {most}]")
+        out.append(np.ascontiguousarray(a, dtype=np.int32))
+    to, of, part = out
+    if of.shape != to.shape or (part is not None and part.shape != to.shape):
+        raise KernelError("copy_pages: lists of different lengths")
+    written = np.zeros(n_dst, dtype=bool)
+    written[to] = True
+    if np.count_nonzero(written) != to.shape[0]:
+        raise KernelError("copy_pages: a page is written twice")
+    if one_pool and written[of].any():
+        raise KernelError("copy_pages: a page is written that is also read")
+    return to, of, part
+
+
+def _shares_memory(a, b) -> bool:
+    """Whether two contiguous tensors overlap; pools that do so have to be one and the same."""
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa == pb and a.shape == b.shape:
+        return True
+    if pa < pb + b.numel() * b.element_size() and pb < pa + a.numel() * a.element_size():
+        raise KernelError("copy_pages: the pools overlap without being one")
+    return False
 
 
 _ERRORS = {-1: "unsupported size, type or option", -2: "bad argument"}
@@ -288,6 +357,11 @@ def _declare(lib) -> None:
                                         I, I, F, I, P, P],
         "hs_moe_sorted_scratch": [I, I, I, I, I, I, P, P],
         "hs_sample": [P, P, P, P, P, P, P, I, I, P, P, P, P],
+        "hs_logit_rules": [P, P, I, I, P, P, P, I, P, P, P, P, P, P, P, I, P, I, P, P, P],
+        "hs_history_begin": [P, P, P, I, I, P, I, P, I, P, P, P, P],
+        "hs_history_add": [P, P, I, I, P, P, I, P, P],
+        "hs_token_logprobs": [P, P, P, P, I, P, P, I, I, P, P],
+        "hs_copy_pages": [P, P, I, P, P, P, I, I, I, I, I, I, P],
     }
     for name, argtypes in sig.items():
         fn = getattr(lib, name)
@@ -2671,3 +2745,190 @@ class CudaOps:
                                   _ptr(seed_lo), _ptr(seed_hi), _ptr(position), rows, vocab,
                                   _ptr(feedback), _ptr(feedback_slot), _ptr(status_word),
                                   self._stream()), "sample")
+
+    # -- rules on logits, and the record of tokens they go by ------------------------------------
+    def _history(self, history, what):
+        """The sizes (slots, vocab) of a record whose tensors belong together."""
+        if not isinstance(history, TokenHistory):
+            raise KernelError(f"{what}: history must be a TokenHistory, "
+                              f"got {type(history).__name__}")
+        prompt, output, counts = history.tensors()
+        for t, nm in ((prompt, "prompt"), (output, "output"), (counts, "counts")):
+            _want(t, f"history.{nm}", torch.int32, 2)
+        n, vocab = counts.shape
+        if prompt.shape != output.shape or tuple(prompt.shape) != (n, history_words(vocab)):
+            raise KernelError(f"{what}: a history of {n} slots and {vocab} tokens with bits of "
+                              f"shapes {tuple(prompt.shape)} and {tuple(output.shape)}")
+        return n, vocab
+
+    def _rows_of(self, what, rows, dtype, **tensors):
+        for nm, t in tensors.items():
+            _want(t, nm, dtype, 1)
+            if t.shape[0] < rows:
+                raise KernelError(f"{what}: {nm} shorter than the rows")
+
+    def _drives(self, t, what):
+        """Kernels run on this object's device, which has to be the current one."""
+        if t.device != self.device or torch.cuda.current_device() != self.device.index:
+            raise KernelError(f"{what}: tensors on {t.device}, current device "
+                              f"{torch.cuda.current_device()}, these kernels drive {self.device}")
+
+    def history_begin(self, history, slots, tokens, start, n_prompt):
+        """For every k: slot ``slots[k]`` gets the record of ``tokens[start[k]:start[k + 1]]``,
+        the first ``n_prompt[k]`` of which are its prompt's and the others generated.  What the
+        slot held before is gone; other slots stay.  A slot below zero is skipped; of two rows
+        of one slot the last counts.  Token ids outside the vocabulary are left out and
+        reported in the status word."""
+        n_slots, vocab = self._history(history, "history_begin")
+        self._drives(history.counts, "history_begin")
+        _want(slots, "slots", torch.int32, 1)
+        rows = slots.shape[0]
+        _want(tokens, "tokens", torch.int32, 1)
+        self._rows_of("history_begin", rows, torch.int32, n_prompt=n_prompt)
+        self._rows_of("history_begin", rows + 1, torch.int32, start=start)
+        self.launches += 1
+        _check(self.lib.hs_history_begin(
+            _ptr(history.prompt), _ptr(history.output), _ptr(history.counts), n_slots, vocab,
+            _ptr(slots), rows, _ptr(tokens), tokens.shape[0], _ptr(start), _ptr(n_prompt),
+            _ptr(self._status_of(slots)), self._stream()), "history_begin")
+
+    def history_add(self, history, slots, tokens):
+        """Count ``tokens[i]`` as generated in slot ``slots[i]`` (below zero: skipped), for as
+        many rows as ``slots`` has."""
+        n_slots, vocab = self._history(history, "history_add")
+        self._drives(history.counts, "history_add")
+        _want(slots, "slots", torch.int32, 1)
+        rows = slots.shape[0]
+        self._rows_of("history_add", rows, torch.int32, tokens=tokens)
+        self.launches += 1
+        _check(self.lib.hs_history_add(
+            _ptr(history.output), _ptr(history.counts), n_slots, vocab, _ptr(slots), _ptr(tokens),
+            rows, _ptr(self._status_of(slots)), self._stream()), "history_add")
+
+    def logit_rules(self, out, logits, history=None, slots=None, repetition=None, presence=None,
+                    frequency=None, *, bias_start=None, bias_ids=None, bias_values=None, mask=None,
+                    mask_row=None):
+        """out = logits under the rules of each row (float32 ``[rows, vocab]``; ``out`` may be
+        ``logits`` itself).  In this order, for token v of row w:
+
+        * seen in the prompt or answer of record ``slots[w]`` (below zero: none): x / repetition
+          where x > 0, else x * repetition;
+        * generated c > 0 times there: less frequency * c + presence;
+        * listed among ``bias_ids[bias_start[w]:bias_start[w + 1]]``: plus its ``bias_values``
+          (of an id listed twice the last entry counts);
+        * bit v % 32 of ``mask[mask_row[w], v // 32]`` unset: -inf (``mask_row`` below zero:
+          no mask).
+
+        The arithmetic on a token is done in 64 bits and rounded once.  Ids, records and masks
+        outside their tables are left out and reported in the status word."""
+        _want(logits, "logits", torch.float32, 2)
+        _want(out, "out", torch.float32, 2)
+        self._drives(logits, "logit_rules")
+        rows, vocab = logits.shape
+        if out.shape != logits.shape:
+            raise KernelError(f"logit_rules: out {tuple(out.shape)} for logits {(rows, vocab)}")
+        a, b, size = out.data_ptr(), logits.data_ptr(), 4 * rows * vocab
+        if a != b and abs(a - b) < size:
+            raise KernelError("logit_rules: out overlaps the logits without being them")
+        n_slots = n_masks = n_bias = 0
+        bits = (None, None, None)
+        if history is not None:
+            n_slots, known = self._history(history, "logit_rules")
+            if known != vocab:
+                raise KernelError(f"logit_rules: a history of {known} tokens for {vocab} logits")
+            self._rows_of("logit_rules", rows, torch.int32, slots=slots)
+            self._rows_of("logit_rules", rows, torch.float32, repetition=repetition,
+                          presence=presence, frequency=frequency)
+            bits = history.tensors()
+        elif not (slots is repetition is presence is frequency is None):
+            raise KernelError("logit_rules: penalties need a history")
+        if bias_start is not None:
+            self._rows_of("logit_rules", rows + 1, torch.int32, bias_start=bias_start)
+            _want(bias_ids, "bias_ids", torch.int32, 1)
+            n_bias = bias_ids.shape[0]
+            self._rows_of("logit_rules", n_bias, torch.float32, bias_values=bias_values)
+            if n_bias == 0:
+                bias_start = None
+        elif not (bias_ids is bias_values is None):
+            raise KernelError("logit_rules: biases need bias_start")
+        if mask is not None:
+            _want(mask, "mask", torch.int32, 2)
+            n_masks = mask.shape[0]
+            if mask.shape[1] != history_words(vocab):
+                raise KernelError(f"logit_rules: mask rows of {mask.shape[1]} words for {vocab} "
+                                  "logits")
+            self._rows_of("logit_rules", rows, torch.int32, mask_row=mask_row)
+            if n_masks == 0:
+                mask = mask_row = None
+        elif mask_row is not None:
+            raise KernelError("logit_rules: mask_row needs a mask")
+        if rows == 0:
+            return
+        self.launches += 1
+        _check(self.lib.hs_logit_rules(
+            a, b, rows, vocab, *map(_ptr, bits), n_slots, _ptr(slots), _ptr(repetition),
+            _ptr(presence), _ptr(frequency), _ptr(bias_start), _ptr(bias_ids), _ptr(bias_values),
+            n_bias, _ptr(mask), n_masks, _ptr(mask_row), _ptr(self._status_of(logits)),
+            self._stream()), f"logit_rules(rows={rows},vocab={vocab})")
+
+    # -- scores -------------------------------------------------------------------------------
+    def token_logprobs(self, logprob, rank, logits, tokens, top_ids=None, top_logprobs=None):
+        """Per row of float32 logits: ``logprob`` of ``tokens[w]`` under their softmax, its
+        ``rank`` (how many tokens stand before it: larger logits, and equal ones of a lower
+        index), and with ``top_ids`` / ``top_logprobs`` ``[rows, n]`` the n tokens that come
+        first in that order.  ``tokens[w] == -1``: no token (logprob NaN, rank -1).  A row of
+        -inf alone has logprobs of -inf, one with a NaN or +inf has NaN."""
+        _want(logits, "logits", torch.float32, 2)
+        self._drives(logits, "token_logprobs")
+        rows, vocab = logits.shape
+        self._rows_of("token_logprobs", rows, torch.float32, logprob=logprob)
+        self._rows_of("token_logprobs", rows, torch.int32, rank=rank, tokens=tokens)
+        top = 0
+        if (top_ids is None) != (top_logprobs is None):
+            raise KernelError("token_logprobs: top_ids and top_logprobs come together")
+        if top_ids is not None:
+            _want(top_ids, "top_ids", torch.int32, 2)
+            _want(top_logprobs, "top_logprobs", torch.float32, 2)
+            top = top_ids.shape[1]
+            if top_ids.shape != top_logprobs.shape or top_ids.shape[0] < rows:
+                raise KernelError(f"token_logprobs: alternatives of shapes {tuple(top_ids.shape)} "
+                                  f"and {tuple(top_logprobs.shape)} for {rows} rows")
+            if top > min(MAX_ALTERNATIVES, vocab):
+                raise KernelError(f"token_logprobs: {top} alternatives; at most "
+                                  f"{min(MAX_ALTERNATIVES, vocab)} of {vocab} tokens")
+        if rows == 0:
+            return
+        self.launches += 1
+        _check(self.lib.hs_token_logprobs(
+            _ptr(logprob), _ptr(rank), _ptr(top_ids), _ptr(top_logprobs), top, _ptr(logits),
+            _ptr(tokens), rows, vocab, _ptr(self._status_of(logits)), self._stream()),
+            f"token_logprobs(rows={rows},vocab={vocab},top={top})")
+
+    # -- pages ----------------------------------------------------------------------------------
+    def copy_pages(self, dst, src, dst_pages, src_pages, rows=None):
+        """``dst[:, dst_pages[i], :, :, :rows[i]] = src[:, src_pages[i], :, :, :rows[i]]`` for
+        every i (``rows`` None: whole pages), for pools ``[entries, pages, planes, kv_heads,
+        page_size, head_dim]`` of one type that differ in their number of pages at most.  The
+        lists are on the host.  Inside one pool no page may be written that is also read, and
+        none twice anywhere: such lists are refused."""
+        _want(dst, "dst", _FLOATS, 6)
+        _want(src, "src", dst.dtype, 6)
+        self._drives(dst, "copy_pages")
+        if src.device != dst.device:
+            raise KernelError("copy_pages: pools on different devices")
+        if dst.shape[0] != src.shape[0] or dst.shape[2:] != src.shape[2:]:
+            raise KernelError(f"copy_pages: pools of shapes {tuple(dst.shape)} and "
+                              f"{tuple(src.shape)}")
+        one_pool = _shares_memory(dst, src)
+        to, of, part = page_lists(dst_pages, src_pages, rows, dst.shape[1], src.shape[1],
+                                  dst.shape[4], one_pool)
+        n = to.shape[0]
+        if n == 0:
+            return
+        entries, _, planes, heads, page_rows, dim = dst.shape
+        self.launches += -(-n // PAGE_LIST)
+        _check(self.lib.hs_copy_pages(
+            dst.data_ptr(), src.data_ptr(), n, to.ctypes.data, of.ctypes.data,
+            None if part is None else part.ctypes.data, entries, dst.shape[1], src.shape[1],
+            planes * heads, page_rows, dim * dst.element_size(), self._stream()),
+            f"copy_pages(n={n},entries={entries})")
