@@ -12,61 +12,175 @@
 
 namespace hs {
 
-constexpr int LR_THREADS = 256, LR_TILE = 4096;
+constexpr int LR_THREADS = 256;
+constexpr int LR_MOST = 8192;             // the widest tile: a word of bits a thread
+constexpr int LR_TILE = 4096;             // of the record's kernel
 
+struct LogitRules {
+  float* out;
+  const float* logits;
+  int vocab, words, tile;
+  const int *prompt, *output, *counts;    // the records
+  int n_slots;
+  const int* slots;
+  const float *repetition, *presence, *frequency;
+  const int *bias_start, *bias_ids;
+  const float* bias_values;
+  int n_bias;
+  const int* mask;
+  int n_masks;
+  const int* mask_row;
+  int* status;
+};
+
+// Bits i .. i + 3 of a row of words (one word more than the row has is readable).
+__device__ __forceinline__ uint32_t lr_four(const uint32_t* words, int i) {
+  return __funnelshift_r(words[i >> 5], words[(i >> 5) + 1], i & 31) & 15u;
+}
+
+// One block a tile of a row.  Most logits are only copied (or ruled out, and then not read at all);
+// the few that stand in the record or are biased are listed first, and computed once the tile has
+// been copied, a thread each, in 64 bits.  In place nothing is copied: only what a rule changes is
+// written.
+template <bool BIAS>
 __global__ void __launch_bounds__(LR_THREADS)
-logit_rules_kernel(float* out, const float* logits, int vocab, int words, const int* prompt,
-                   const int* output, const int* counts, int n_slots, const int* slots,
-                   const float* repetition, const float* presence, const float* frequency,
-                   const int* bias_start, const int* bias_ids, const float* bias_values, int n_bias,
-                   const int* mask, int n_masks, const int* mask_row, int* status) {
+logit_rules_kernel(const LogitRules a) {
+  __shared__ uint32_t s_seen[LR_MOST / 32], s_said[LR_MOST / 32], s_mask[LR_MOST / 32 + 1];
+  __shared__ uint16_t s_list[LR_MOST];
+  __shared__ int s_n;
+  extern __shared__ int s_entry[];        // [tile], BIAS only: the bias entry of a token, or -1
   pdl_trigger();
   pdl_wait();
-  const int w = blockIdx.y;
-  const int slot = slots ? slots[w] : -1;
-  const bool known = slot >= 0 && slot < n_slots;
-  const int mrow = mask ? mask_row[w] : -1;
-  const bool masked = mrow >= 0 && mrow < n_masks;
-  if (blockIdx.x == 0 && threadIdx.x == 0 && (slot >= n_slots || mrow >= n_masks) && (slots || mask))
-    if ((slots && slot >= n_slots) || (mask && mrow >= n_masks)) atomicOr(status, HS_STATUS_BAD_ROW);
+  const int w = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  const int lo = blockIdx.x * a.tile, n = min(a.vocab - lo, a.tile), n_words = (n + 31) / 32;
+  const int slot = a.slots ? a.slots[w] : -1, mrow = a.mask ? a.mask_row[w] : -1;
+  const bool known = slot >= 0 && slot < a.n_slots, masked = mrow >= 0 && mrow < a.n_masks;
   int b0 = 0, b1 = 0;
-  if (bias_start) {
-    b0 = max(0, bias_start[w]);
-    b1 = min(n_bias, bias_start[w + 1]);
+  if (BIAS) {
+    b0 = max(0, a.bias_start[w]);
+    b1 = min(a.n_bias, a.bias_start[w + 1]);
   }
-  const int lo = blockIdx.x * LR_TILE, hi = min(vocab, lo + LR_TILE);
-  for (int v = lo + threadIdx.x; v < hi; v += LR_THREADS) {
-    const size_t at = (size_t)w * vocab + v;
-    const uint32_t bit = 1u << (v & 31);
-    float x = logits[at];
-    double y = x;
-    bool changed = false;
+  if (tid == 0) {
+    s_n = 0;
+    if (blockIdx.x == 0 && (slot >= a.n_slots || mrow >= a.n_masks) &&
+        ((a.slots && slot >= a.n_slots) || (a.mask && mrow >= a.n_masks)))
+      atomicOr(a.status, HS_STATUS_BAD_ROW);
+  }
+  uint32_t seen = 0, said = 0;
+  if (tid < n_words) {
+    const size_t word = (size_t)(lo >> 5) + tid;
     if (known) {
-      const size_t word = (size_t)slot * words + (v >> 5);
-      const bool said = (uint32_t)output[word] & bit;
-      if (said || ((uint32_t)prompt[word] & bit)) {
-        const double r = repetition[w];
-        y = y > 0. ? y / r : y * r;
-        if (said) {
-          const int c = counts[(size_t)slot * vocab + v];
-          y -= (double)frequency[w] * c + (c > 0 ? (double)presence[w] : 0.);
-        }
-        changed = true;
+      said = (uint32_t)a.output[(size_t)slot * a.words + word];
+      seen = (uint32_t)a.prompt[(size_t)slot * a.words + word] | said;
+      const int left = n - 32 * tid;      // (bits behind the vocabulary say nothing)
+      if (left < 32) seen &= (1u << left) - 1u;
+    }
+    s_seen[tid] = seen;
+    s_said[tid] = said;
+    s_mask[tid] = masked ? (uint32_t)a.mask[(size_t)mrow * a.words + word] : 0xffffffffu;
+  }
+  if (tid == 0) s_mask[n_words] = 0;
+  if (BIAS && b1 > b0)
+    for (int i = tid; i < n; i += LR_THREADS) s_entry[i] = -1;
+  __syncthreads();
+  if (BIAS && b1 > b0) {
+    for (int j = b0 + tid; j < b1; j += LR_THREADS) {
+      const int v = a.bias_ids[j], i = v - lo;
+      if (v < 0 || v >= a.vocab) {
+        if (blockIdx.x == 0) atomicOr(a.status, HS_STATUS_BAD_TOKEN);
+      } else if (i >= 0 && i < n) {
+        atomicMax(&s_entry[i], j);
+        atomicOr(&s_seen[i >> 5], 1u << (i & 31));
       }
     }
-    for (int j = b1 - 1; j >= b0; --j)
-      if (bias_ids[j] == v) {
-        y += bias_values[j];
-        changed = true;
-        break;
-      }
-    if (changed) x = (float)y;
-    if (masked && !((uint32_t)mask[(size_t)mrow * words + (v >> 5)] & bit)) x = -INFINITY;
-    out[at] = x;
+    __syncthreads();
+    if (tid < n_words) seen = s_seen[tid];
   }
-  if (blockIdx.x == 0)
-    for (int j = b0 + threadIdx.x; j < b1; j += LR_THREADS)
-      if (bias_ids[j] < 0 || bias_ids[j] >= vocab) atomicOr(status, HS_STATUS_BAD_TOKEN);
+  // list what has to be computed: ruled-out tokens need not be
+  uint32_t todo = tid < n_words ? seen & s_mask[tid] : 0u;
+  if (__any_sync(0xffffffffu, todo != 0u)) {
+    const int c = __popc(todo);
+    int incl = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
+    }
+    int at = 0;
+    if (lane == 31) at = atomicAdd(&s_n, incl);
+    at = __shfl_sync(0xffffffffu, at, 31) + incl - c;
+    for (uint32_t bits = todo; bits; bits &= bits - 1) s_list[at++] = (uint16_t)(32 * tid + __ffs(bits) - 1);
+  }
+
+  const size_t first = (size_t)w * a.vocab + lo;
+  const float* from = a.logits + first;
+  float* to = a.out + first;
+  const bool in_place = from == to;
+  const int off = (int)(((uintptr_t)from >> 2) & 3);
+  if ((((uintptr_t)from ^ (uintptr_t)to) & 15) == 0) {
+    // pieces of four that begin on 16 bytes: piece p holds the places 4 p - off + 0..3
+    const int pieces = (n + off + 3) / 4;
+    if (!in_place || masked) {
+      constexpr int INFLIGHT = 4;
+      for (int p0 = tid; p0 < pieces; p0 += INFLIGHT * LR_THREADS) {
+        float4 x[INFLIGHT];
+        uint32_t keep[INFLIGHT];
+#pragma unroll
+        for (int k = 0; k < INFLIGHT; ++k) {
+          const int i = 4 * (p0 + k * LR_THREADS) - off;
+          keep[k] = 0u;
+          x[k] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+          if (i >= 0 && i + 3 < n) {
+            keep[k] = masked ? lr_four(s_mask, i) : 15u;
+            if (keep[k] != 0u && !(in_place && keep[k] == 15u)) x[k] = *(const float4*)(from + i);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < INFLIGHT; ++k) {
+          const int i = 4 * (p0 + k * LR_THREADS) - off;
+          if (i >= 0 && i + 3 < n) {
+            if (in_place && keep[k] == 15u) continue;
+            if (!(keep[k] & 1u)) x[k].x = -INFINITY;
+            if (!(keep[k] & 2u)) x[k].y = -INFINITY;
+            if (!(keep[k] & 4u)) x[k].z = -INFINITY;
+            if (!(keep[k] & 8u)) x[k].w = -INFINITY;
+            *(float4*)(to + i) = x[k];
+          } else if (p0 + k * LR_THREADS < pieces) {
+            for (int j = max(i, 0); j < min(i + 4, n); ++j) {
+              const bool kept = (s_mask[j >> 5] >> (j & 31)) & 1u;
+              if (!in_place || !kept) to[j] = kept ? from[j] : -INFINITY;
+            }
+          }
+        }
+      }
+    }
+  } else {
+    for (int j = tid; j < n; j += LR_THREADS) to[j] = (s_mask[j >> 5] >> (j & 31)) & 1u ? from[j] : -INFINITY;
+  }
+  __syncthreads();
+  const int listed = s_n;
+  for (int l = tid; l < listed; l += LR_THREADS) {
+    const int i = s_list[l];
+    double y = from[i];
+    if (known) {
+      const uint32_t bit = 1u << (i & 31);
+      const bool out_bit = s_said[i >> 5] & bit;
+      // (a bit that only the bias set is not in the record)
+      if (out_bit || !BIAS || ((uint32_t)a.prompt[(size_t)slot * a.words + ((lo + i) >> 5)] & bit)) {
+        const double r = a.repetition[w];
+        y = y > 0. ? y / r : y * r;
+        if (out_bit) {
+          const int c = a.counts[(size_t)slot * a.vocab + lo + i];
+          y -= (double)a.frequency[w] * c + (c > 0 ? (double)a.presence[w] : 0.);
+        }
+      }
+    }
+    if (BIAS && b1 > b0) {
+      const int j = s_entry[i];
+      if (j >= 0) y += a.bias_values[j];
+    }
+    to[i] = (float)y;
+  }
 }
 
 // One block a tile of the vocabulary and slot: the tile's counts are formed in shared memory from
@@ -85,23 +199,29 @@ history_begin_kernel(int* prompt, int* output, int* counts, int vocab, int words
     if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(status, HS_STATUS_BAD_ROW);
     return;
   }
-  for (int j = k + 1; j < n_rows; ++j)      // of two rows of one slot the last counts
-    if (slots[j] == slot) return;
+  // of two rows of one slot the last counts
+  bool again = false;
+  for (int j = k + 1 + threadIdx.x; j < n_rows; j += LR_THREADS) again |= slots[j] == slot;
   const int lo = blockIdx.x * LR_TILE;
   for (int i = threadIdx.x; i < LR_TILE; i += LR_THREADS) s_count[i] = 0;
   for (int i = threadIdx.x; i < LR_TILE / 32; i += LR_THREADS) s_prompt[i] = 0;
-  __syncthreads();
+  if (__syncthreads_or(again)) return;
   const int t0 = max(0, start[k]), t1 = min(n_tokens, start[k + 1]), p1 = start[k] + n_prompt[k];
-  for (int t = t0 + threadIdx.x; t < t1; t += LR_THREADS) {
-    const int v = tokens[t];
-    if (v < 0 || v >= vocab) {
-      if (blockIdx.x == 0) atomicOr(status, HS_STATUS_BAD_TOKEN);
-      continue;
+  constexpr int INFLIGHT = 8;
+  for (int t = t0 + threadIdx.x; t < t1; t += INFLIGHT * LR_THREADS) {
+    int v[INFLIGHT];
+#pragma unroll
+    for (int j = 0; j < INFLIGHT; ++j) v[j] = t + j * LR_THREADS < t1 ? tokens[t + j * LR_THREADS] : lo - 1;
+#pragma unroll
+    for (int j = 0; j < INFLIGHT; ++j) {
+      const int i = v[j] - lo;
+      if (i >= 0 && i < LR_TILE && v[j] < vocab) {
+        if (t + j * LR_THREADS < p1) atomicOr(&s_prompt[i >> 5], 1u << (i & 31));
+        else atomicAdd(&s_count[i], 1);
+      } else if (blockIdx.x == 0 && t + j * LR_THREADS < t1 && (v[j] < 0 || v[j] >= vocab)) {
+        atomicOr(status, HS_STATUS_BAD_TOKEN);
+      }
     }
-    const int i = v - lo;
-    if (i < 0 || i >= LR_TILE) continue;
-    if (t < p1) atomicOr(&s_prompt[i >> 5], 1u << (i & 31));
-    else atomicAdd(&s_count[i], 1);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < LR_TILE; i += LR_THREADS) {
@@ -150,11 +270,19 @@ HS_EXPORT int hs_logit_rules(float* out, const float* logits, int rows, int voca
   if ((mask == nullptr) != (mask_row == nullptr)) return HS_ERR_ARGUMENT;
   if (rows <= 0) return HS_OK;
   if (rows > 65535) return HS_ERR_UNSUPPORTED;
-  const cudaError_t e = hs_launch(
-      hs::logit_rules_kernel, dim3((vocab + hs::LR_TILE - 1) / hs::LR_TILE, rows), dim3(hs::LR_THREADS),
-      0, (cudaStream_t)stream, hs_pdl_enabled(), out, logits, vocab, (vocab + 31) / 32, prompt, output,
-      counts, n_slots, slots, repetition, presence, frequency, bias_start, bias_ids, bias_values, n_bias,
-      mask, n_masks, mask_row, status);
+  // the widest tile that still gives every SM four blocks (with biases a word a token beside it)
+  const int most = bias_start ? hs::LR_MOST / 2 : hs::LR_MOST;
+  int tile = 1024;
+  while (tile < most && (long long)rows * ((vocab + 2 * tile - 1) / (2 * tile)) >= 4 * 148) tile *= 2;
+  const hs::LogitRules args{out, logits, vocab, (vocab + 31) / 32, tile, prompt, output, counts, n_slots,
+                            slots, repetition, presence, frequency, bias_start, bias_ids, bias_values,
+                            n_bias, mask, n_masks, mask_row, status};
+  const dim3 grid((vocab + tile - 1) / tile, rows);
+  const cudaError_t e =
+      bias_start ? hs_launch(hs::logit_rules_kernel<true>, grid, dim3(hs::LR_THREADS),
+                             tile * sizeof(int), (cudaStream_t)stream, hs_pdl_enabled(), args)
+                 : hs_launch(hs::logit_rules_kernel<false>, grid, dim3(hs::LR_THREADS), 0,
+                             (cudaStream_t)stream, hs_pdl_enabled(), args);
   return e == cudaSuccess ? HS_OK : (int)e;
 }
 
