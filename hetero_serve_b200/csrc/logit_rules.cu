@@ -14,7 +14,7 @@ namespace hs {
 
 constexpr int LR_THREADS = 256;
 constexpr int LR_MOST = 8192;             // the widest tile: a word of bits a thread
-constexpr int LR_TILE = 4096;             // of the record's kernel
+constexpr int LH_THREADS = 512, LH_TILE = 8192;    // of the record's kernel
 
 struct LogitRules {
   float* out;
@@ -45,10 +45,11 @@ __device__ __forceinline__ uint32_t lr_four(const uint32_t* words, int i) {
 template <bool BIAS>
 __global__ void __launch_bounds__(LR_THREADS)
 logit_rules_kernel(const LogitRules a) {
-  __shared__ uint32_t s_seen[LR_MOST / 32], s_said[LR_MOST / 32], s_mask[LR_MOST / 32 + 1];
+  __shared__ uint32_t s_seen[LR_MOST / 32];      // in the record, or biased
+  __shared__ uint32_t s_known[LR_MOST / 32], s_said[LR_MOST / 32], s_mask[LR_MOST / 32 + 1];
   __shared__ uint16_t s_list[LR_MOST];
   __shared__ int s_n;
-  extern __shared__ int s_entry[];        // [tile], BIAS only: the bias entry of a token, or -1
+  extern __shared__ __align__(16) int s_entry[];        // [tile], BIAS only: the bias entry of a token, or -1
   pdl_trigger();
   pdl_wait();
   const int w = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
@@ -66,6 +67,26 @@ logit_rules_kernel(const LogitRules a) {
         ((a.slots && slot >= a.n_slots) || (a.mask && mrow >= a.n_masks)))
       atomicOr(a.status, HS_STATUS_BAD_ROW);
   }
+  const size_t first = (size_t)w * a.vocab + lo;
+  const float* from = a.logits + first;
+  float* to = a.out + first;
+  const bool in_place = from == to;
+  const int off = (int)(((uintptr_t)from >> 2) & 3);
+  const bool even = (((uintptr_t)from ^ (uintptr_t)to) & 15) == 0;
+  // pieces of four that begin on 16 bytes: piece p holds the places 4 p - off + 0..3.  Where every
+  // logit is copied, the first of them are under way while the record is read.
+  const int pieces = even ? (n + off + 3) / 4 : 0;
+  const bool ahead = !in_place && !masked;
+  constexpr int INFLIGHT = 4;
+  float4 x[INFLIGHT];
+  if (ahead) {
+#pragma unroll
+    for (int k = 0; k < INFLIGHT; ++k) {
+      const int i = 4 * (tid + k * LR_THREADS) - off;
+      if (i >= 0 && i + 3 < n && even) x[k] = *(const float4*)(from + i);
+    }
+  }
+
   uint32_t seen = 0, said = 0;
   if (tid < n_words) {
     const size_t word = (size_t)(lo >> 5) + tid;
@@ -76,12 +97,13 @@ logit_rules_kernel(const LogitRules a) {
       if (left < 32) seen &= (1u << left) - 1u;
     }
     s_seen[tid] = seen;
+    s_known[tid] = seen;
     s_said[tid] = said;
     s_mask[tid] = masked ? (uint32_t)a.mask[(size_t)mrow * a.words + word] : 0xffffffffu;
   }
   if (tid == 0) s_mask[n_words] = 0;
   if (BIAS && b1 > b0)
-    for (int i = tid; i < n; i += LR_THREADS) s_entry[i] = -1;
+    for (int i = tid; i < (n + 3) / 4; i += LR_THREADS) ((int4*)s_entry)[i] = make_int4(-1, -1, -1, -1);
   __syncthreads();
   if (BIAS && b1 > b0) {
     for (int j = b0 + tid; j < b1; j += LR_THREADS) {
@@ -112,49 +134,38 @@ logit_rules_kernel(const LogitRules a) {
     for (uint32_t bits = todo; bits; bits &= bits - 1) s_list[at++] = (uint16_t)(32 * tid + __ffs(bits) - 1);
   }
 
-  const size_t first = (size_t)w * a.vocab + lo;
-  const float* from = a.logits + first;
-  float* to = a.out + first;
-  const bool in_place = from == to;
-  const int off = (int)(((uintptr_t)from >> 2) & 3);
-  if ((((uintptr_t)from ^ (uintptr_t)to) & 15) == 0) {
-    // pieces of four that begin on 16 bytes: piece p holds the places 4 p - off + 0..3
-    const int pieces = (n + off + 3) / 4;
-    if (!in_place || masked) {
-      constexpr int INFLIGHT = 4;
-      for (int p0 = tid; p0 < pieces; p0 += INFLIGHT * LR_THREADS) {
-        float4 x[INFLIGHT];
-        uint32_t keep[INFLIGHT];
+  if (even && (!in_place || masked)) {
+    for (int p0 = tid; p0 < pieces; p0 += INFLIGHT * LR_THREADS) {
+      uint32_t keep[INFLIGHT];
 #pragma unroll
-        for (int k = 0; k < INFLIGHT; ++k) {
-          const int i = 4 * (p0 + k * LR_THREADS) - off;
-          keep[k] = 0u;
-          x[k] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-          if (i >= 0 && i + 3 < n) {
-            keep[k] = masked ? lr_four(s_mask, i) : 15u;
-            if (keep[k] != 0u && !(in_place && keep[k] == 15u)) x[k] = *(const float4*)(from + i);
-          }
+      for (int k = 0; k < INFLIGHT; ++k) {
+        const int i = 4 * (p0 + k * LR_THREADS) - off;
+        keep[k] = 15u;
+        if (i >= 0 && i + 3 < n) {
+          if (masked) keep[k] = lr_four(s_mask, i);
+          if (keep[k] != 0u && !(in_place && keep[k] == 15u) && !(ahead && p0 == tid))
+            x[k] = *(const float4*)(from + i);
         }
+      }
 #pragma unroll
-        for (int k = 0; k < INFLIGHT; ++k) {
-          const int i = 4 * (p0 + k * LR_THREADS) - off;
-          if (i >= 0 && i + 3 < n) {
-            if (in_place && keep[k] == 15u) continue;
-            if (!(keep[k] & 1u)) x[k].x = -INFINITY;
-            if (!(keep[k] & 2u)) x[k].y = -INFINITY;
-            if (!(keep[k] & 4u)) x[k].z = -INFINITY;
-            if (!(keep[k] & 8u)) x[k].w = -INFINITY;
-            *(float4*)(to + i) = x[k];
-          } else if (p0 + k * LR_THREADS < pieces) {
-            for (int j = max(i, 0); j < min(i + 4, n); ++j) {
-              const bool kept = (s_mask[j >> 5] >> (j & 31)) & 1u;
-              if (!in_place || !kept) to[j] = kept ? from[j] : -INFINITY;
-            }
+      for (int k = 0; k < INFLIGHT; ++k) {
+        const int i = 4 * (p0 + k * LR_THREADS) - off;
+        if (i >= 0 && i + 3 < n) {
+          if (in_place && keep[k] == 15u) continue;
+          if (!(keep[k] & 1u)) x[k].x = -INFINITY;
+          if (!(keep[k] & 2u)) x[k].y = -INFINITY;
+          if (!(keep[k] & 4u)) x[k].z = -INFINITY;
+          if (!(keep[k] & 8u)) x[k].w = -INFINITY;
+          *(float4*)(to + i) = x[k];
+        } else if (p0 + k * LR_THREADS < pieces) {
+          for (int j = max(i, 0); j < min(i + 4, n); ++j) {
+            const bool kept = (s_mask[j >> 5] >> (j & 31)) & 1u;
+            if (!in_place || !kept) to[j] = kept ? from[j] : -INFINITY;
           }
         }
       }
     }
-  } else {
+  } else if (!even) {
     for (int j = tid; j < n; j += LR_THREADS) to[j] = (s_mask[j >> 5] >> (j & 31)) & 1u ? from[j] : -INFINITY;
   }
   __syncthreads();
@@ -165,8 +176,7 @@ logit_rules_kernel(const LogitRules a) {
     if (known) {
       const uint32_t bit = 1u << (i & 31);
       const bool out_bit = s_said[i >> 5] & bit;
-      // (a bit that only the bias set is not in the record)
-      if (out_bit || !BIAS || ((uint32_t)a.prompt[(size_t)slot * a.words + ((lo + i) >> 5)] & bit)) {
+      if (s_known[i >> 5] & bit) {
         const double r = a.repetition[w];
         y = y > 0. ? y / r : y * r;
         if (out_bit) {
@@ -183,55 +193,64 @@ logit_rules_kernel(const LogitRules a) {
   }
 }
 
-// One block a tile of the vocabulary and slot: the tile's counts are formed in shared memory from
-// all of the slot's tokens and written whole, so that nothing has to be cleared first.
-__global__ void __launch_bounds__(LR_THREADS)
+// One block a tile of the vocabulary and slot: the tile's bits and counts are formed in shared memory
+// from all of the slot's tokens and written whole, so that nothing has to be cleared first.
+__global__ void __launch_bounds__(LH_THREADS)
 history_begin_kernel(int* prompt, int* output, int* counts, int vocab, int words, int n_slots,
                      const int* slots, int n_rows, const int* tokens, int n_tokens, const int* start,
                      const int* n_prompt, int* status) {
-  __shared__ int s_count[LR_TILE];
-  __shared__ uint32_t s_prompt[LR_TILE / 32];
+  __shared__ int4 s_count4[LH_TILE / 4 + 1];
+  __shared__ uint32_t s_bits[2][LH_TILE / 32];
+  int* s_count = (int*)s_count4;
   pdl_trigger();
   pdl_wait();
-  const int k = blockIdx.y, slot = slots[k];
+  const int k = blockIdx.y, tid = threadIdx.x, slot = slots[k];
   if (slot < 0) return;
   if (slot >= n_slots) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(status, HS_STATUS_BAD_ROW);
+    if (blockIdx.x == 0 && tid == 0) atomicOr(status, HS_STATUS_BAD_ROW);
     return;
   }
+  const int t0 = max(0, start[k]), t1 = min(n_tokens, start[k + 1]), p1 = start[k] + n_prompt[k];
   // of two rows of one slot the last counts
   bool again = false;
-  for (int j = k + 1 + threadIdx.x; j < n_rows; j += LR_THREADS) again |= slots[j] == slot;
-  const int lo = blockIdx.x * LR_TILE;
-  for (int i = threadIdx.x; i < LR_TILE; i += LR_THREADS) s_count[i] = 0;
-  for (int i = threadIdx.x; i < LR_TILE / 32; i += LR_THREADS) s_prompt[i] = 0;
+  for (int j = k + 1 + tid; j < n_rows; j += LH_THREADS) again |= slots[j] == slot;
+  for (int i = tid; i < LH_TILE / 4 + 1; i += LH_THREADS) s_count4[i] = make_int4(0, 0, 0, 0);
+  if (tid < 2 * LH_TILE / 32) (&s_bits[0][0])[tid] = 0u;
   if (__syncthreads_or(again)) return;
-  const int t0 = max(0, start[k]), t1 = min(n_tokens, start[k + 1]), p1 = start[k] + n_prompt[k];
+  const int lo = blockIdx.x * LH_TILE, n = min(LH_TILE, vocab - lo);
+  int* to = counts + (size_t)slot * vocab + lo;
+  const int off = (int)(((uintptr_t)to >> 2) & 3);      // counts stand as they do in their row's pieces
   constexpr int INFLIGHT = 8;
-  for (int t = t0 + threadIdx.x; t < t1; t += INFLIGHT * LR_THREADS) {
+  for (int t = t0 + tid; t < t1; t += INFLIGHT * LH_THREADS) {
     int v[INFLIGHT];
 #pragma unroll
-    for (int j = 0; j < INFLIGHT; ++j) v[j] = t + j * LR_THREADS < t1 ? tokens[t + j * LR_THREADS] : lo - 1;
+    for (int j = 0; j < INFLIGHT; ++j) v[j] = t + j * LH_THREADS < t1 ? tokens[t + j * LH_THREADS] : 0;
 #pragma unroll
     for (int j = 0; j < INFLIGHT; ++j) {
-      const int i = v[j] - lo;
-      if (i >= 0 && i < LR_TILE && v[j] < vocab) {
-        if (t + j * LR_THREADS < p1) atomicOr(&s_prompt[i >> 5], 1u << (i & 31));
-        else atomicAdd(&s_count[i], 1);
-      } else if (blockIdx.x == 0 && t + j * LR_THREADS < t1 && (v[j] < 0 || v[j] >= vocab)) {
+      const int at = t + j * LH_THREADS, i = v[j] - lo;
+      if (at >= t1) break;
+      if (v[j] >= lo && i < n) {
+        const bool said = at >= p1;
+        if (said) atomicAdd(&s_count[off + i], 1);
+        atomicOr(&s_bits[said][i >> 5], 1u << (i & 31));
+      } else if (blockIdx.x == 0 && (v[j] < 0 || v[j] >= vocab)) {
         atomicOr(status, HS_STATUS_BAD_TOKEN);
       }
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < LR_TILE; i += LR_THREADS) {
-    const int v = lo + i;
-    const int c = s_count[i];
-    const uint32_t said = __ballot_sync(0xffffffffu, c > 0);
-    if (v < vocab) counts[(size_t)slot * vocab + v] = c;
-    if ((i & 31) == 0 && (v >> 5) < words) {
-      output[(size_t)slot * words + (v >> 5)] = (int)said;
-      prompt[(size_t)slot * words + (v >> 5)] = (int)s_prompt[i >> 5];
+  if (tid < (n + 31) / 32) {
+    const size_t word = (size_t)slot * words + (lo >> 5) + tid;
+    prompt[word] = (int)s_bits[0][tid];
+    output[word] = (int)s_bits[1][tid];
+  }
+  const int pieces = (n + off + 3) / 4;
+  for (int p = tid; p < pieces; p += LH_THREADS) {
+    const int i = 4 * p - off;
+    if (i >= 0 && i + 3 < n) {
+      *(int4*)(to + i) = s_count4[p];
+    } else {
+      for (int j = max(i, 0); j < min(i + 4, n); ++j) to[j] = s_count[off + j];
     }
   }
 }
@@ -297,8 +316,8 @@ HS_EXPORT int hs_history_begin(int* prompt, int* output, int* counts, int n_slot
   if (n_rows <= 0) return HS_OK;
   if (n_rows > 65535) return HS_ERR_UNSUPPORTED;
   const cudaError_t e = hs_launch(
-      hs::history_begin_kernel, dim3((vocab + hs::LR_TILE - 1) / hs::LR_TILE, n_rows),
-      dim3(hs::LR_THREADS), 0, (cudaStream_t)stream, hs_pdl_enabled(), prompt, output, counts, vocab,
+      hs::history_begin_kernel, dim3((vocab + hs::LH_TILE - 1) / hs::LH_TILE, n_rows),
+      dim3(hs::LH_THREADS), 0, (cudaStream_t)stream, hs_pdl_enabled(), prompt, output, counts, vocab,
       (vocab + 31) / 32, n_slots, slots, n_rows, tokens, n_tokens, start, n_prompt, status);
   return e == cudaSuccess ? HS_OK : (int)e;
 }

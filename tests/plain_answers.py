@@ -13,10 +13,6 @@ from plain_ops import PlainOps
 WORD = 32
 
 
-def get_bit(words, v):
-    return (int(words[v // WORD]) >> (v % WORD)) & 1
-
-
 def set_bit(words, v):
     value = (int(words[v // WORD]) & 0xFFFFFFFF) | (1 << (v % WORD))
     words[v // WORD] = value - (1 << 32) if value >= 1 << 31 else value
@@ -29,6 +25,12 @@ def pack(flags):
     for r, v in torch.nonzero(flags.cpu()).tolist():
         set_bit(out[r], v)
     return out
+
+
+def bits_set(words):
+    """The indices of the set bits of one row of words."""
+    return [WORD * i + b for i, word in enumerate(words.tolist()) if word
+            for b in range(WORD) if (word >> b) & 1]
 
 
 class PlainAnswerOps(PlainOps):
@@ -66,13 +68,14 @@ class PlainAnswerOps(PlainOps):
         y = logits.double().clone()
         for w in range(rows):
             slot = -1 if history is None else int(slots[w])
-            if 0 <= slot < history.counts.shape[0] if history is not None else False:
-                for v in range(vocab):
-                    said = get_bit(history.output[slot], v)
-                    if said or get_bit(history.prompt[slot], v):
-                        r = float(repetition[w])
-                        y[w, v] = y[w, v] / r if y[w, v] > 0 else y[w, v] * r
-                    if said:
+            if history is not None and 0 <= slot < history.counts.shape[0]:
+                said = set(bits_set(history.output[slot]))
+                for v in said | set(bits_set(history.prompt[slot])):
+                    if v >= vocab:
+                        continue
+                    r = float(repetition[w])
+                    y[w, v] = y[w, v] / r if y[w, v] > 0 else y[w, v] * r
+                    if v in said:
                         c = int(history.counts[slot, v])
                         y[w, v] -= float(frequency[w]) * c + (float(presence[w]) if c else 0.0)
             if bias_start is not None:
@@ -83,9 +86,10 @@ class PlainAnswerOps(PlainOps):
                     if 0 <= v < vocab:
                         y[w, v] += b
             if mask is not None and 0 <= int(mask_row[w]) < mask.shape[0]:
-                for v in range(vocab):
-                    if not get_bit(mask[int(mask_row[w])], v):
-                        y[w, v] = -math.inf
+                kept = [v for v in bits_set(mask[int(mask_row[w])]) if v < vocab]
+                ruled = torch.full((vocab,), -math.inf, dtype=torch.float64)
+                ruled[kept] = y[w, kept]
+                y[w] = ruled
         out.copy_(y.to(out.dtype))
 
     def token_logprobs(self, logprob, rank, logits, tokens, top_ids=None, top_logprobs=None):

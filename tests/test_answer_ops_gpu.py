@@ -179,6 +179,10 @@ def check_rules(ops, s, in_place=False):
     (2, 50257, dict(bias=100, mask=0.5)),
     (40, 517, dict(bias=9, mask=0.9)),
     (700, 65, dict(bias=2, mask=0.6)),
+    (90, 13001, dict(bias=3)),
+    (90, 13001, dict(mask=0.7)),
+    (310, 9001, dict()),
+    (310, 9001, dict(bias=5, mask=0.05)),
 ])
 def test_rules_follow_the_plain_form(ops, rows, vocab, kw, in_place):
     gen = torch.Generator().manual_seed(rows * 131 + vocab)
