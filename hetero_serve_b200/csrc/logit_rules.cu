@@ -12,8 +12,9 @@
 
 namespace hs {
 
-constexpr int LR_THREADS = 256;
+constexpr int LR_THREADS = 256, LR_BLOCKS = 6;     // of a block; of an SM
 constexpr int LR_MOST = 8192;             // the widest tile: a word of bits a thread
+constexpr int LR_BIASES = 512;            // biases of a tile that are kept at hand
 constexpr int LH_THREADS = 512, LH_TILE = 8192;    // of the record's kernel
 
 struct LogitRules {
@@ -43,13 +44,16 @@ __device__ __forceinline__ uint32_t lr_four(const uint32_t* words, int i) {
 // been copied, a thread each, in 64 bits.  In place nothing is copied: only what a rule changes is
 // written.
 template <bool BIAS>
-__global__ void __launch_bounds__(LR_THREADS)
+__global__ void __launch_bounds__(LR_THREADS, LR_BLOCKS)
 logit_rules_kernel(const LogitRules a) {
   __shared__ uint32_t s_seen[LR_MOST / 32];      // in the record, or biased
   __shared__ uint32_t s_known[LR_MOST / 32], s_said[LR_MOST / 32], s_mask[LR_MOST / 32 + 1];
   __shared__ uint16_t s_list[LR_MOST];
   __shared__ int s_n;
-  extern __shared__ __align__(16) int s_entry[];        // [tile], BIAS only: the bias entry of a token, or -1
+  // (place in the tile, bias entry) in any order; where they are too many, the last entry of each of
+  // so many places at a time
+  __shared__ int2 s_entry[BIAS ? LR_BIASES : 1];
+  __shared__ int s_entries;
   pdl_trigger();
   pdl_wait();
   const int w = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
@@ -62,7 +66,7 @@ logit_rules_kernel(const LogitRules a) {
     b1 = min(a.n_bias, a.bias_start[w + 1]);
   }
   if (tid == 0) {
-    s_n = 0;
+    s_n = s_entries = 0;
     if (blockIdx.x == 0 && (slot >= a.n_slots || mrow >= a.n_masks) &&
         ((a.slots && slot >= a.n_slots) || (a.mask && mrow >= a.n_masks)))
       atomicOr(a.status, HS_STATUS_BAD_ROW);
@@ -102,16 +106,17 @@ logit_rules_kernel(const LogitRules a) {
     s_mask[tid] = masked ? (uint32_t)a.mask[(size_t)mrow * a.words + word] : 0xffffffffu;
   }
   if (tid == 0) s_mask[n_words] = 0;
-  if (BIAS && b1 > b0)
-    for (int i = tid; i < (n + 3) / 4; i += LR_THREADS) ((int4*)s_entry)[i] = make_int4(-1, -1, -1, -1);
+  int entry_id = -1;                      // the first round of the row's biases
+  if (BIAS && b0 + tid < b1) entry_id = a.bias_ids[b0 + tid];
   __syncthreads();
   if (BIAS && b1 > b0) {
     for (int j = b0 + tid; j < b1; j += LR_THREADS) {
-      const int v = a.bias_ids[j], i = v - lo;
+      const int v = j == b0 + tid ? entry_id : a.bias_ids[j], i = v - lo;
       if (v < 0 || v >= a.vocab) {
         if (blockIdx.x == 0) atomicOr(a.status, HS_STATUS_BAD_TOKEN);
       } else if (i >= 0 && i < n) {
-        atomicMax(&s_entry[i], j);
+        const int at = atomicAdd(&s_entries, 1);
+        if (at < LR_BIASES) s_entry[at] = make_int2(i, j);
         atomicOr(&s_seen[i >> 5], 1u << (i & 31));
       }
     }
@@ -170,26 +175,46 @@ logit_rules_kernel(const LogitRules a) {
   }
   __syncthreads();
   const int listed = s_n;
-  for (int l = tid; l < listed; l += LR_THREADS) {
-    const int i = s_list[l];
+  auto compute = [&](int i, int entry) {
     double y = from[i];
-    if (known) {
-      const uint32_t bit = 1u << (i & 31);
-      const bool out_bit = s_said[i >> 5] & bit;
-      if (s_known[i >> 5] & bit) {
-        const double r = a.repetition[w];
-        y = y > 0. ? y / r : y * r;
-        if (out_bit) {
-          const int c = a.counts[(size_t)slot * a.vocab + lo + i];
-          y -= (double)a.frequency[w] * c + (c > 0 ? (double)a.presence[w] : 0.);
-        }
+    const uint32_t bit = 1u << (i & 31);
+    if (known && (s_known[i >> 5] & bit)) {
+      const double r = a.repetition[w];
+      y = y > 0. ? y / r : y * r;
+      if (s_said[i >> 5] & bit) {
+        const int c = a.counts[(size_t)slot * a.vocab + lo + i];
+        y -= (double)a.frequency[w] * c + (c > 0 ? (double)a.presence[w] : 0.);
       }
     }
-    if (BIAS && b1 > b0) {
-      const int j = s_entry[i];
-      if (j >= 0) y += a.bias_values[j];
-    }
+    if (BIAS && entry >= 0) y += a.bias_values[entry];
     to[i] = (float)y;
+  };
+  if (!BIAS || s_entries <= LR_BIASES) {
+    const int entries = BIAS ? s_entries : 0;
+    for (int l = tid; l < listed; l += LR_THREADS) {
+      const int i = s_list[l];
+      int last = -1;
+      for (int e = 0; e < entries; ++e)
+        if (s_entry[e].x == i) last = max(last, s_entry[e].y);
+      compute(i, last);
+    }
+  } else {
+    constexpr int PLACES = 2 * LR_BIASES;
+    int* s_last = (int*)s_entry;
+    for (int from_place = 0; from_place < n; from_place += PLACES) {
+      __syncthreads();
+      for (int i = tid; i < PLACES; i += LR_THREADS) s_last[i] = -1;
+      __syncthreads();
+      for (int j = b0 + tid; j < b1; j += LR_THREADS) {
+        const unsigned i = (unsigned)a.bias_ids[j] - (unsigned)(lo + from_place);
+        if (i < PLACES) atomicMax(&s_last[i], j);
+      }
+      __syncthreads();
+      for (int l = tid; l < listed; l += LR_THREADS) {
+        const int i = s_list[l];
+        if (i >= from_place && i < from_place + PLACES) compute(i, s_last[i - from_place]);
+      }
+    }
   }
 }
 
@@ -289,17 +314,17 @@ HS_EXPORT int hs_logit_rules(float* out, const float* logits, int rows, int voca
   if ((mask == nullptr) != (mask_row == nullptr)) return HS_ERR_ARGUMENT;
   if (rows <= 0) return HS_OK;
   if (rows > 65535) return HS_ERR_UNSUPPORTED;
-  // the widest tile that still gives every SM four blocks (with biases a word a token beside it)
-  const int most = bias_start ? hs::LR_MOST / 2 : hs::LR_MOST;
-  int tile = 1024;
-  while (tile < most && (long long)rows * ((vocab + 2 * tile - 1) / (2 * tile)) >= 4 * 148) tile *= 2;
+  // as many tiles as run at a time, none narrower than a round of a block's loads
+  const int fit = hs::LR_BLOCKS * hs_sm_count(), tiles = fit / rows > 1 ? fit / rows : 1;
+  int tile = ((vocab + tiles - 1) / tiles + 1023) / 1024 * 1024;
+  if (tile > hs::LR_MOST) tile = hs::LR_MOST;
   const hs::LogitRules args{out, logits, vocab, (vocab + 31) / 32, tile, prompt, output, counts, n_slots,
                             slots, repetition, presence, frequency, bias_start, bias_ids, bias_values,
                             n_bias, mask, n_masks, mask_row, status};
   const dim3 grid((vocab + tile - 1) / tile, rows);
   const cudaError_t e =
-      bias_start ? hs_launch(hs::logit_rules_kernel<true>, grid, dim3(hs::LR_THREADS),
-                             tile * sizeof(int), (cudaStream_t)stream, hs_pdl_enabled(), args)
+      bias_start ? hs_launch(hs::logit_rules_kernel<true>, grid, dim3(hs::LR_THREADS), 0,
+                             (cudaStream_t)stream, hs_pdl_enabled(), args)
                  : hs_launch(hs::logit_rules_kernel<false>, grid, dim3(hs::LR_THREADS), 0,
                              (cudaStream_t)stream, hs_pdl_enabled(), args);
   return e == cudaSuccess ? HS_OK : (int)e;

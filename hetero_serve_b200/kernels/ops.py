@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 from ctypes import c_float, c_int, c_void_p
 from dataclasses import dataclass
 
@@ -134,7 +135,7 @@ class FusedTables:
         return self.data.data_ptr() + self.n_layers * self.layer_bytes
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class TokenHistory:
     """Which tokens the request in each state slot holds, in device memory: what penalties for
     repeated tokens go by.  ``prompt`` and ``output`` are bits over the vocabulary (bit v % 32
@@ -144,6 +145,15 @@ class TokenHistory:
     prompt: torch.Tensor          # [slots, words] int32
     output: torch.Tensor          # [slots, words] int32
     counts: torch.Tensor          # [slots, vocab] int32
+
+    def __post_init__(self):
+        for nm in ("prompt", "output", "counts"):
+            _want(getattr(self, nm), f"history.{nm}", torch.int32, 2, cuda=False)
+        slots, vocab = self.counts.shape
+        for t in (self.prompt, self.output):
+            if tuple(t.shape) != (slots, history_words(vocab)) or t.device != self.counts.device:
+                raise KernelError(f"a history of {slots} slots and {vocab} tokens on "
+                                  f"{self.counts.device} with bits {tuple(t.shape)} on {t.device}")
 
     @classmethod
     def zeros(cls, slots: int, vocab: int, device) -> "TokenHistory":
@@ -196,31 +206,53 @@ def plan_decode_ints(n_rows: int) -> int:
 PAGE_LIST = 1024          # pages a launch of the page copy takes
 
 
+def _whole_numbers(given, name, least, most) -> array:
+    """A list (or array) of whole numbers between two bounds as C ints."""
+    try:
+        if isinstance(given, np.ndarray):
+            if given.ndim != 1 or given.dtype.kind not in "iu":
+                raise TypeError
+            if given.size and not (least <= int(given.min()) and int(given.max()) <= most):
+                raise OverflowError
+            return array("i", given.astype(np.int32).tobytes())
+        out = array("i", given)
+        if len(out) > 64:
+            view = np.frombuffer(out, dtype=np.int32)
+            low, high = int(view.min()), int(view.max())
+        elif out:
+            low, high = min(out), max(out)
+        else:
+            return out
+        if low < least or high > most:
+            raise OverflowError
+        return out
+    except TypeError:
+        raise KernelError(f"copy_pages: {name}: a list of whole numbers wanted") from None
+    except OverflowError:
+        raise KernelError(f"copy_pages: {name}: a number lies outside [{least}, {most}]") from None
+
+
 def page_lists(dst_pages, src_pages, rows, n_dst, n_src, page_rows, one_pool):
-    """The lists of a page copy as int32 arrays (``rows`` may be None).  Refused are lists of
+    """The lists of a page copy as arrays of C ints (``rows`` may be None).  Refused are lists of
     different lengths or of anything but whole numbers, that reach outside their pools, write a
     page twice, or, inside one pool, write a page that is also read."""
-    out = []
-    for nm, given, least, most in (("written", dst_pages, 0, n_dst - 1),
-                                   ("read", src_pages, 0, n_src - 1),
-                                   ("filled rows", rows, 0, page_rows)):
-        if given is None:
-            out.append(None)
-            continue
-        a = np.asarray(given)
-        if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
-            raise KernelError(f"copy_pages: {nm}: a list of whole numbers wanted")
-        if a.size and (int(a.min()) < least or int(a.max()) > most):
-            raise KernelError(f"copy_pages: {nm}: a number lies outside [{least}, {most}]")
-        out.append(np.ascontiguousarray(a, dtype=np.int32))
-    to, of, part = out
-    if of.shape != to.shape or (part is not None and part.shape != to.shape):
+    to = _whole_numbers(dst_pages, "pages written", 0, n_dst - 1)
+    of = _whole_numbers(src_pages, "pages read", 0, n_src - 1)
+    part = None if rows is None else _whole_numbers(rows, "filled rows", 0, page_rows)
+    n = len(to)
+    if len(of) != n or (part is not None and len(part) != n):
         raise KernelError("copy_pages: lists of different lengths")
-    written = np.zeros(n_dst, dtype=bool)
-    written[to] = True
-    if np.count_nonzero(written) != to.shape[0]:
+    if n <= 64:
+        written = set(to)
+        twice, also = len(written) != n, one_pool and not written.isdisjoint(of)
+    else:
+        marks = np.zeros(n_dst, dtype=bool)
+        marks[np.frombuffer(to, dtype=np.int32)] = True
+        twice = np.count_nonzero(marks) != n
+        also = one_pool and bool(marks[np.frombuffer(of, dtype=np.int32)].any())
+    if twice:
         raise KernelError("copy_pages: a page is written twice")
-    if one_pool and written[of].any():
+    if also:
         raise KernelError("copy_pages: a page is written that is also read")
     return to, of, part
 
@@ -494,7 +526,8 @@ class CudaOps:
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
 
     def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
+        # (the stream's handle without a Stream object around it, which costs 2 us a launch)
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
 
     # -- kernels that parts bring themselves -------------------------------------------
     def stream(self) -> int:
@@ -2747,31 +2780,33 @@ class CudaOps:
                                   self._stream()), "sample")
 
     # -- rules on logits, and the record of tokens they go by ------------------------------------
-    def _history(self, history, what):
-        """The sizes (slots, vocab) of a record whose tensors belong together."""
+    def _fits(self, what, t, name, dtype, rows):
+        """Refuse anything but a vector of ``rows`` numbers or more on this object's device."""
+        if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == 1
+                and t.get_device() == self.device.index and t.is_contiguous()
+                and t.numel() >= rows):
+            return
+        _want(t, name, dtype, 1)
+        if t.numel() < rows:
+            raise KernelError(f"{what}: {name} shorter than the rows")
+        self._drives(what, t)
+
+    def _drives(self, what, *tensors):
+        """Kernels run on this object's device, which has to be the current one."""
+        for t in tensors:
+            if t.device != self.device:
+                raise KernelError(f"{what}: a tensor on {t.device}; these kernels drive "
+                                  f"{self.device}")
+        if torch.cuda.current_device() != self.device.index:
+            raise KernelError(f"{what}: device {torch.cuda.current_device()} is current; these "
+                              f"kernels drive {self.device}")
+
+    def _history(self, what, history):
         if not isinstance(history, TokenHistory):
             raise KernelError(f"{what}: history must be a TokenHistory, "
                               f"got {type(history).__name__}")
-        prompt, output, counts = history.tensors()
-        for t, nm in ((prompt, "prompt"), (output, "output"), (counts, "counts")):
-            _want(t, f"history.{nm}", torch.int32, 2)
-        n, vocab = counts.shape
-        if prompt.shape != output.shape or tuple(prompt.shape) != (n, history_words(vocab)):
-            raise KernelError(f"{what}: a history of {n} slots and {vocab} tokens with bits of "
-                              f"shapes {tuple(prompt.shape)} and {tuple(output.shape)}")
-        return n, vocab
-
-    def _rows_of(self, what, rows, dtype, **tensors):
-        for nm, t in tensors.items():
-            _want(t, nm, dtype, 1)
-            if t.shape[0] < rows:
-                raise KernelError(f"{what}: {nm} shorter than the rows")
-
-    def _drives(self, t, what):
-        """Kernels run on this object's device, which has to be the current one."""
-        if t.device != self.device or torch.cuda.current_device() != self.device.index:
-            raise KernelError(f"{what}: tensors on {t.device}, current device "
-                              f"{torch.cuda.current_device()}, these kernels drive {self.device}")
+        self._drives(what, history.counts)
+        return history.counts.shape
 
     def history_begin(self, history, slots, tokens, start, n_prompt):
         """For every k: slot ``slots[k]`` gets the record of ``tokens[start[k]:start[k + 1]]``,
@@ -2779,13 +2814,13 @@ class CudaOps:
         slot held before is gone; other slots stay.  A slot below zero is skipped; of two rows
         of one slot the last counts.  Token ids outside the vocabulary are left out and
         reported in the status word."""
-        n_slots, vocab = self._history(history, "history_begin")
-        self._drives(history.counts, "history_begin")
-        _want(slots, "slots", torch.int32, 1)
+        what = "history_begin"
+        n_slots, vocab = self._history(what, history)
+        self._fits(what, slots, "slots", torch.int32, 0)
         rows = slots.shape[0]
-        _want(tokens, "tokens", torch.int32, 1)
-        self._rows_of("history_begin", rows, torch.int32, n_prompt=n_prompt)
-        self._rows_of("history_begin", rows + 1, torch.int32, start=start)
+        self._fits(what, tokens, "tokens", torch.int32, 0)
+        self._fits(what, n_prompt, "n_prompt", torch.int32, rows)
+        self._fits(what, start, "start", torch.int32, rows + 1)
         self.launches += 1
         _check(self.lib.hs_history_begin(
             _ptr(history.prompt), _ptr(history.output), _ptr(history.counts), n_slots, vocab,
@@ -2795,11 +2830,11 @@ class CudaOps:
     def history_add(self, history, slots, tokens):
         """Count ``tokens[i]`` as generated in slot ``slots[i]`` (below zero: skipped), for as
         many rows as ``slots`` has."""
-        n_slots, vocab = self._history(history, "history_add")
-        self._drives(history.counts, "history_add")
-        _want(slots, "slots", torch.int32, 1)
+        what = "history_add"
+        n_slots, vocab = self._history(what, history)
+        self._fits(what, slots, "slots", torch.int32, 0)
         rows = slots.shape[0]
-        self._rows_of("history_add", rows, torch.int32, tokens=tokens)
+        self._fits(what, tokens, "tokens", torch.int32, rows)
         self.launches += 1
         _check(self.lib.hs_history_add(
             _ptr(history.output), _ptr(history.counts), n_slots, vocab, _ptr(slots), _ptr(tokens),
@@ -2821,43 +2856,47 @@ class CudaOps:
 
         The arithmetic on a token is done in 64 bits and rounded once.  Ids, records and masks
         outside their tables are left out and reported in the status word."""
+        what = "logit_rules"
         _want(logits, "logits", torch.float32, 2)
         _want(out, "out", torch.float32, 2)
-        self._drives(logits, "logit_rules")
+        self._drives(what, logits, out)
         rows, vocab = logits.shape
         if out.shape != logits.shape:
             raise KernelError(f"logit_rules: out {tuple(out.shape)} for logits {(rows, vocab)}")
-        a, b, size = out.data_ptr(), logits.data_ptr(), 4 * rows * vocab
-        if a != b and abs(a - b) < size:
+        a, b = out.data_ptr(), logits.data_ptr()
+        if a != b and abs(a - b) < 4 * rows * vocab:
             raise KernelError("logit_rules: out overlaps the logits without being them")
         n_slots = n_masks = n_bias = 0
         bits = (None, None, None)
         if history is not None:
-            n_slots, known = self._history(history, "logit_rules")
+            n_slots, known = self._history(what, history)
             if known != vocab:
                 raise KernelError(f"logit_rules: a history of {known} tokens for {vocab} logits")
-            self._rows_of("logit_rules", rows, torch.int32, slots=slots)
-            self._rows_of("logit_rules", rows, torch.float32, repetition=repetition,
-                          presence=presence, frequency=frequency)
-            bits = history.tensors()
+            self._fits(what, slots, "slots", torch.int32, rows)
+            self._fits(what, repetition, "repetition", torch.float32, rows)
+            self._fits(what, presence, "presence", torch.float32, rows)
+            self._fits(what, frequency, "frequency", torch.float32, rows)
+            bits = (history.prompt.data_ptr(), history.output.data_ptr(),
+                    history.counts.data_ptr())
         elif not (slots is repetition is presence is frequency is None):
             raise KernelError("logit_rules: penalties need a history")
         if bias_start is not None:
-            self._rows_of("logit_rules", rows + 1, torch.int32, bias_start=bias_start)
-            _want(bias_ids, "bias_ids", torch.int32, 1)
+            self._fits(what, bias_start, "bias_start", torch.int32, rows + 1)
+            self._fits(what, bias_ids, "bias_ids", torch.int32, 0)
             n_bias = bias_ids.shape[0]
-            self._rows_of("logit_rules", n_bias, torch.float32, bias_values=bias_values)
+            self._fits(what, bias_values, "bias_values", torch.float32, n_bias)
             if n_bias == 0:
                 bias_start = None
         elif not (bias_ids is bias_values is None):
             raise KernelError("logit_rules: biases need bias_start")
         if mask is not None:
             _want(mask, "mask", torch.int32, 2)
+            self._drives(what, mask)
             n_masks = mask.shape[0]
             if mask.shape[1] != history_words(vocab):
                 raise KernelError(f"logit_rules: mask rows of {mask.shape[1]} words for {vocab} "
                                   "logits")
-            self._rows_of("logit_rules", rows, torch.int32, mask_row=mask_row)
+            self._fits(what, mask_row, "mask_row", torch.int32, rows)
             if n_masks == 0:
                 mask = mask_row = None
         elif mask_row is not None:
@@ -2866,7 +2905,7 @@ class CudaOps:
             return
         self.launches += 1
         _check(self.lib.hs_logit_rules(
-            a, b, rows, vocab, *map(_ptr, bits), n_slots, _ptr(slots), _ptr(repetition),
+            a, b, rows, vocab, *bits, n_slots, _ptr(slots), _ptr(repetition),
             _ptr(presence), _ptr(frequency), _ptr(bias_start), _ptr(bias_ids), _ptr(bias_values),
             n_bias, _ptr(mask), n_masks, _ptr(mask_row), _ptr(self._status_of(logits)),
             self._stream()), f"logit_rules(rows={rows},vocab={vocab})")
@@ -2878,17 +2917,20 @@ class CudaOps:
         index), and with ``top_ids`` / ``top_logprobs`` ``[rows, n]`` the n tokens that come
         first in that order.  ``tokens[w] == -1``: no token (logprob NaN, rank -1).  A row of
         -inf alone has logprobs of -inf, one with a NaN or +inf has NaN."""
+        what = "token_logprobs"
         _want(logits, "logits", torch.float32, 2)
-        self._drives(logits, "token_logprobs")
+        self._drives(what, logits)
         rows, vocab = logits.shape
-        self._rows_of("token_logprobs", rows, torch.float32, logprob=logprob)
-        self._rows_of("token_logprobs", rows, torch.int32, rank=rank, tokens=tokens)
+        self._fits(what, logprob, "logprob", torch.float32, rows)
+        self._fits(what, rank, "rank", torch.int32, rows)
+        self._fits(what, tokens, "tokens", torch.int32, rows)
         top = 0
         if (top_ids is None) != (top_logprobs is None):
             raise KernelError("token_logprobs: top_ids and top_logprobs come together")
         if top_ids is not None:
             _want(top_ids, "top_ids", torch.int32, 2)
             _want(top_logprobs, "top_logprobs", torch.float32, 2)
+            self._drives(what, top_ids, top_logprobs)
             top = top_ids.shape[1]
             if top_ids.shape != top_logprobs.shape or top_ids.shape[0] < rows:
                 raise KernelError(f"token_logprobs: alternatives of shapes {tuple(top_ids.shape)} "
@@ -2913,22 +2955,20 @@ class CudaOps:
         none twice anywhere: such lists are refused."""
         _want(dst, "dst", _FLOATS, 6)
         _want(src, "src", dst.dtype, 6)
-        self._drives(dst, "copy_pages")
-        if src.device != dst.device:
-            raise KernelError("copy_pages: pools on different devices")
+        self._drives("copy_pages", dst, src)
         if dst.shape[0] != src.shape[0] or dst.shape[2:] != src.shape[2:]:
             raise KernelError(f"copy_pages: pools of shapes {tuple(dst.shape)} and "
                               f"{tuple(src.shape)}")
         one_pool = _shares_memory(dst, src)
         to, of, part = page_lists(dst_pages, src_pages, rows, dst.shape[1], src.shape[1],
                                   dst.shape[4], one_pool)
-        n = to.shape[0]
+        n = len(to)
         if n == 0:
             return
         entries, _, planes, heads, page_rows, dim = dst.shape
         self.launches += -(-n // PAGE_LIST)
         _check(self.lib.hs_copy_pages(
-            dst.data_ptr(), src.data_ptr(), n, to.ctypes.data, of.ctypes.data,
-            None if part is None else part.ctypes.data, entries, dst.shape[1], src.shape[1],
+            dst.data_ptr(), src.data_ptr(), n, to.buffer_info()[0], of.buffer_info()[0],
+            None if part is None else part.buffer_info()[0], entries, dst.shape[1], src.shape[1],
             planes * heads, page_rows, dim * dst.element_size(), self._stream()),
             f"copy_pages(n={n},entries={entries})")

@@ -183,6 +183,8 @@ def check_rules(ops, s, in_place=False):
     (90, 13001, dict(mask=0.7)),
     (310, 9001, dict()),
     (310, 9001, dict(bias=5, mask=0.05)),
+    (2, 4099, dict(bias=6000, mask=0.5)),        # more biases than a tile keeps at hand
+    (130, 9001, dict(bias=3000)),
 ])
 def test_rules_follow_the_plain_form(ops, rows, vocab, kw, in_place):
     gen = torch.Generator().manual_seed(rows * 131 + vocab)

@@ -1,6 +1,7 @@
 """What the operations around a step's answers refuse, without a GPU: the lists of page copies on
 the host; the checks of tensors on an object whose library stands in for the CUDA one."""
 
+import numpy as np
 import pytest
 import torch
 
@@ -31,7 +32,7 @@ def ops(monkeypatch):
     o.device, o.lib, o.launches = torch.device("cpu"), NoLibrary(), 0
     o.status = torch.zeros(1, dtype=torch.int32)
     monkeypatch.setattr(CudaOps, "_stream", lambda self: 0)
-    monkeypatch.setattr(CudaOps, "_drives", lambda self, t, what: None)
+    monkeypatch.setattr(CudaOps, "_drives", lambda self, what, *tensors: None)
     return o
 
 
@@ -63,7 +64,23 @@ def test_page_lists_that_are_refused(to, of, rows, one, why):
 def test_page_lists_that_are_taken():
     to, of, rows = page_lists([3, 0], [3, 3], [0, 16], 10, 8, 16, False)
     assert to.tolist() == [3, 0] and of.tolist() == [3, 3] and rows.tolist() == [0, 16]
-    assert page_lists([], [], None, 10, 10, 16, True)[0].shape == (0,)
+    assert len(page_lists([], [], None, 10, 10, 16, True)[0]) == 0
+    many = np.arange(400)
+    for kind in (many, many.tolist(), many.astype(np.uint16), torch.arange(400)):
+        to, of, rows = page_lists(kind, many + 400, many % 17, 800, 800, 16, True)
+        assert to.tolist() == many.tolist() and of.tolist() == (many + 400).tolist()
+        assert rows.tolist() == (many % 17).tolist()
+
+
+@pytest.mark.parametrize("many,why", [
+    (np.arange(400) % 399, "written twice"), (np.arange(400) - 1, "outside"),
+    (np.arange(400) + 401, "outside"), (np.arange(400) + 2 ** 32, "outside"),
+    (np.arange(400) + 0.0, "whole numbers"), (np.arange(400) + 1, "also read"),
+])
+def test_long_page_lists_that_are_refused(many, why):
+    for kind in (many, many.tolist()):
+        with pytest.raises(KernelError, match=why):
+            page_lists(kind, np.arange(400) + 400, None, 800, 800, 16, True)
 
 
 def test_page_copies_refuse_pools_that_do_not_match(ops):
@@ -90,8 +107,6 @@ def test_rules_refuse_what_does_not_fit(ops):
     bad = [dict(full, slots=i32(2)), dict(full, slots=None), dict(full, repetition=f[:2]),
            dict(full, presence=f.double()), dict(full, frequency=None),
            dict(full, history=TokenHistory.zeros(4, 99, "cpu")),
-           dict(full, history=TokenHistory(h.prompt, h.output[:3], h.counts)),
-           dict(full, history=TokenHistory(h.prompt, h.output, h.counts.float())),
            dict(full, history=h.counts), dict(slots=i32(3)),
            dict(bias_start=i32(3), bias_ids=i32(2), bias_values=torch.zeros(2)),
            dict(bias_start=i32(4), bias_ids=i32(2), bias_values=torch.zeros(1)),
@@ -101,6 +116,10 @@ def test_rules_refuse_what_does_not_fit(ops):
     for kw in bad:
         with pytest.raises(KernelError):
             ops.logit_rules(out, x, **kw)
+    for parts in ((h.prompt, h.output[:3], h.counts), (h.prompt, h.output, h.counts.float()),
+                  (h.prompt[:, :3].contiguous(), h.output, h.counts), (h.prompt, None, h.counts)):
+        with pytest.raises(KernelError):
+            TokenHistory(*parts)
     for o, l in ((out[:2], x), (out.double(), x), (torch.zeros(100, 3).T, x), (out, x.bfloat16())):
         with pytest.raises(KernelError):
             ops.logit_rules(o, l)
