@@ -9,17 +9,19 @@
 
 namespace hs {
 
-constexpr int PC_THREADS = 256, PC_PAIRS = 1024;
+constexpr int PC_THREADS = 256;
+constexpr int PC_FEW = 32, PC_MANY = 1024;     // pairs a launch takes
 
+template <int PAIRS>
 struct PageList {
-  int dst[PC_PAIRS], src[PC_PAIRS];
-  short rows[PC_PAIRS];
+  int dst[PAIRS], src[PAIRS];
+  short rows[PAIRS];
 };
 
-template <typename V>
+template <typename V, int PAIRS>
 __global__ void __launch_bounds__(PC_THREADS)
 copy_pages_kernel(V* dst, const V* src, long long dst_pages, long long src_pages, int tiles,
-                  int page_rows, int row_vecs, const __grid_constant__ PageList list) {
+                  int page_rows, int row_vecs, const __grid_constant__ PageList<PAIRS> list) {
   pdl_trigger();
   pdl_wait();
   const int i = blockIdx.x, e = blockIdx.y;
@@ -34,19 +36,19 @@ copy_pages_kernel(V* dst, const V* src, long long dst_pages, long long src_pages
   }
 }
 
-template <typename V>
+template <typename V, int PAIRS>
 cudaError_t copy_pages(void* dst, const void* src, int n, const int* dst_list, const int* src_list,
                        const int* rows, int entries, int dst_pages, int src_pages, int tiles,
                        int page_rows, int row_bytes, cudaStream_t stream) {
-  for (int from = 0; from < n; from += PC_PAIRS) {
-    const int count = n - from < PC_PAIRS ? n - from : PC_PAIRS;
-    PageList list;
+  for (int from = 0; from < n; from += PAIRS) {
+    const int count = n - from < PAIRS ? n - from : PAIRS;
+    PageList<PAIRS> list;
     for (int i = 0; i < count; ++i) {
       list.dst[i] = dst_list[from + i];
       list.src[i] = src_list[from + i];
       list.rows[i] = (short)(rows ? rows[from + i] : page_rows);
     }
-    const cudaError_t e = hs_launch(copy_pages_kernel<V>, dim3(count, entries), dim3(PC_THREADS), 0,
+    const cudaError_t e = hs_launch(copy_pages_kernel<V, PAIRS>, dim3(count, entries), dim3(PC_THREADS), 0,
                                     stream, hs_pdl_enabled(), (V*)dst, (const V*)src,
                                     (long long)dst_pages, (long long)src_pages, tiles, page_rows,
                                     (int)(row_bytes / sizeof(V)), list);
@@ -74,14 +76,15 @@ HS_EXPORT int hs_copy_pages(void* dst, const void* src, int n, const int* dst_li
   const uintptr_t bits = (uintptr_t)dst | (uintptr_t)src | (uintptr_t)row_bytes;
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
-  if (bits % 16 == 0)
-    e = hs::copy_pages<uint4>(dst, src, n, dst_list, src_list, rows, entries, dst_pages, src_pages,
-                              tiles, page_rows, row_bytes, st);
-  else if (bits % 4 == 0)
-    e = hs::copy_pages<uint32_t>(dst, src, n, dst_list, src_list, rows, entries, dst_pages, src_pages,
-                                 tiles, page_rows, row_bytes, st);
-  else
-    e = hs::copy_pages<uint16_t>(dst, src, n, dst_list, src_list, rows, entries, dst_pages, src_pages,
-                                 tiles, page_rows, row_bytes, st);
+#define PC_GO(V)                                                                                     \
+  e = n <= hs::PC_FEW                                                                                \
+          ? hs::copy_pages<V, hs::PC_FEW>(dst, src, n, dst_list, src_list, rows, entries, dst_pages, \
+                                          src_pages, tiles, page_rows, row_bytes, st)                \
+          : hs::copy_pages<V, hs::PC_MANY>(dst, src, n, dst_list, src_list, rows, entries, dst_pages, \
+                                           src_pages, tiles, page_rows, row_bytes, st)
+  if (bits % 16 == 0) PC_GO(uint4);
+  else if (bits % 4 == 0) PC_GO(uint32_t);
+  else PC_GO(uint16_t);
+#undef PC_GO
   return e == cudaSuccess ? HS_OK : (int)e;
 }

@@ -6,28 +6,33 @@
 // A row that is -inf throughout has no probabilities: every lp is -inf.  A NaN or +inf in a row makes
 // all of its lp NaN; in the order a NaN stands behind everything else.
 //
-// One pass over the row: every thread keeps a running maximum with the sum of exp against it, counts
-// the logits before x_t, and remembers which of its pieces held its maximum.  The n largest of the
-// row lie in the n threads whose maxima are the largest (each of those threads holds one at least as
-// large as the n-th of them), so that only their logits are looked at again: n / threads of the row.
+// One pass over the row: every thread keeps a running maximum with the sum of exp against it, and
+// counts the logits before x_t.  For the alternatives the threads form 32 groups: the n-th largest of
+// the groups' maxima is a bound that at least n logits reach, and not many more (about 30 of a row of
+// any length for n = 20).  Only the threads whose own maximum reaches the bound look at their logits
+// again, the block together; what they find is put in order by counting.  Where too many logits are
+// equal for that (a row of zeros, of -inf), or NaNs leave too few, the threads' largest logits are
+// ordered with their indices instead, which bounds what is looked at whatever the values are.
 // A row is shared by the blocks of a cluster where there are few rows.
 #include "common.cuh"
 
 namespace hs {
 
 constexpr int TL_TOP = 32;                // a warp's lanes hold the alternatives, in order
+constexpr int TL_GROUPS = 32;             // of threads, whose maxima give the bound
 constexpr int TL_INFLIGHT = 4;            // 16-byte loads a thread has under way
-constexpr int TL_CAND = 4096;             // logits looked at again at a time
+constexpr int TL_CAND = 1024;             // logits looked at again at a time
 
 typedef unsigned long long tl_key_t;
 
 // order of (logit, index): larger logits first, among equal ones the lower index; zeros of both
 // signs are equal, NaN is the smallest; 0 stands for no logit at all
+__device__ __forceinline__ uint32_t tl_order(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return x != x ? 0u : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
 __device__ __forceinline__ tl_key_t tl_key(float x, int v) {
-  uint32_t b = __float_as_uint(x + 0.f);
-  b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  if (x != x) b = 0u;
-  return ((tl_key_t)b << 32) | (uint32_t)~(uint32_t)v;
+  return ((tl_key_t)tl_order(x) << 32) | (uint32_t)~(uint32_t)v;
 }
 __device__ __forceinline__ float tl_value(tl_key_t key) {
   const uint32_t b = (uint32_t)(key >> 32);
@@ -56,17 +61,48 @@ __device__ __forceinline__ tl_key_t tl_merged(tl_key_t a, tl_key_t b_reversed, i
   return k;
 }
 
+// 2^x, to two steps; what lies below the range of normal numbers is 0 (beside a sum of 1 or more)
+__device__ __forceinline__ float tl_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float TL_LOG2E = 1.4426950408889634f;
+
 // A running maximum and the sum of exp against it.  Nothing is subtracted from an infinite maximum:
 // -inf stands for no logit yet (every term is then 0), +inf makes the sum NaN by itself.
 struct TlSum {
   float m, s;
 };
 __device__ __forceinline__ float tl_term(float x, float m) {
-  return __expf(x - (m == -INFINITY ? 0.f : m));
+  return tl_exp2((x - (m == -INFINITY ? 0.f : m)) * TL_LOG2E);
 }
 __device__ __forceinline__ TlSum tl_join(TlSum a, TlSum b) {
   const float m = fmaxf(a.m, b.m);
   return TlSum{m, a.s * tl_term(a.m, m) + b.s * tl_term(b.m, m)};
+}
+
+// two numbers at a time
+typedef unsigned long long tl_pair;
+__device__ __forceinline__ tl_pair tl_two(float a, float b) {
+  tl_pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ float2 tl_apart(tl_pair p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+__device__ __forceinline__ tl_pair tl_add(tl_pair a, tl_pair b) {
+  tl_pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ tl_pair tl_mul(tl_pair a, tl_pair b) {
+  tl_pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 __device__ __forceinline__ uint32_t tl_rank() {
@@ -97,42 +133,35 @@ __device__ __forceinline__ T tl_remote(const T* p, int rank) {
   }
 }
 
-// A row as pieces of four logits that begin on 16 bytes: piece p holds the indices 4 p - off + 0..3;
-// places outside the row read as -inf.
-struct TlRow {
-  const float* row;
-  int vocab, off;
-  __device__ __forceinline__ float4 load(int p) const {
-    const int v = 4 * p - off;
-    if (v >= 0 && v + 3 < vocab) return *(const float4*)(row + v);
-    float x[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = v + j >= 0 && v + j < vocab ? row[v + j] : -INFINITY;
-    return make_float4(x[0], x[1], x[2], x[3]);
-  }
-};
-
 template <int THREADS, int BLOCKS>
 __global__ void __launch_bounds__(THREADS)
 token_logprobs_kernel(float* __restrict__ logprob, int* __restrict__ rank, int* __restrict__ top_ids,
                       float* __restrict__ top_logprobs, int top, const float* __restrict__ logits,
                       const int* __restrict__ tokens, int vocab, int* status) {
-  constexpr int WARPS = THREADS / 32;
+  constexpr int WARPS = THREADS / 32, STEP = TL_INFLIGHT * THREADS;
+  static_assert(THREADS >= 2 * TL_GROUPS && THREADS >= BLOCKS * TL_TOP && BLOCKS * TL_TOP <= TL_CAND, "");
   __shared__ TlSum s_sum[WARPS];
   __shared__ int s_before[WARPS];
+  __shared__ __align__(16) uint32_t s_group[TL_GROUPS];
   __shared__ tl_key_t s_list[WARPS][TL_TOP];
-  __shared__ int s_found;
-  __shared__ TlSum s_block;             // what the cluster's first block reads of the others
-  __shared__ int s_block_before;
+  __shared__ tl_key_t s_top[TL_TOP];    // the block's alternatives, in order
+  __shared__ uint16_t s_owner[THREADS];
+  __shared__ int s_owners, s_found, s_block_before;
+  __shared__ TlSum s_block;
   extern __shared__ tl_key_t s_cand[];  // [TL_CAND] where alternatives are wanted
   pdl_trigger();
   pdl_wait();
   const int w = blockIdx.x / BLOCKS, part = BLOCKS > 1 ? (int)tl_rank() : 0;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // a row is up to three logits, pieces of four that begin on 16 bytes, and up to three logits
   const float* base = logits + (size_t)w * vocab;
-  const TlRow row{base, vocab, (int)(((uintptr_t)base >> 2) & 3)};
-  const int pieces = (vocab + row.off + 3) / 4, per = (pieces + BLOCKS - 1) / BLOCKS;
+  const int head = min(vocab, (int)((4 - (((uintptr_t)base >> 2) & 3)) & 3));
+  const int pieces = (vocab - head) / 4, tail = (vocab - head) % 4;
+  const int per = (pieces + BLOCKS - 1) / BLOCKS;
   const int p0 = min(pieces, part * per), p1 = min(pieces, p0 + per);
+  const float4* row = (const float4*)(base + head);
+  // the logits outside the pieces: a thread each, of the first block
+  const int edge = part != 0 || tid >= head + tail ? -1 : tid < head ? tid : head + 4 * pieces + tid - head;
 
   const int t = tokens[w];
   const bool given = t >= 0 && t < vocab;
@@ -144,66 +173,61 @@ token_logprobs_kernel(float* __restrict__ logprob, int* __restrict__ rank, int* 
   const tl_key_t mine = given ? tl_key(xt, t) : ~0ull;
 
   TlSum own{-INFINITY, 0.f};
-  int before = 0, best_at = p0 + tid;
-  for (int p = p0 + tid; p < p1; p += TL_INFLIGHT * THREADS) {
-    float x[TL_INFLIGHT][4];
+  int before = 0;
+  if (edge >= 0) {
+    const float x = base[edge];
+    own = TlSum{fmaxf(x, -INFINITY), x != x ? x : x == -INFINITY ? 0.f : tl_term(x, x)};
+    before = tl_key(x, edge) > mine;
+  }
+  float m_pieces = -INFINITY;             // the largest in the thread's pieces
+  auto chunk = [&](int at, bool whole) {  // pieces at + tid, + THREADS, ...
+    float4 f[TL_INFLIGHT];
 #pragma unroll
     for (int i = 0; i < TL_INFLIGHT; ++i) {
-      float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      if (p + i * THREADS < p1) f = row.load(p + i * THREADS);
-      x[i][0] = f.x; x[i][1] = f.y; x[i][2] = f.z; x[i][3] = f.w;
+      f[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      if (whole || at + tid + i * THREADS < p1) f[i] = row[at + tid + i * THREADS];
     }
     float m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < TL_INFLIGHT; ++i)
-      m = fmaxf(m, fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3])));
+      m = fmaxf(fmaxf(fmaxf(m, f[i].x), f[i].y), fmaxf(f[i].z, f[i].w));
+    m_pieces = fmaxf(m_pieces, m);
     if (m > own.m) {
       own.s *= tl_term(own.m, m);
       own.m = m;
-      best_at = p;
     }
-    const float ref = own.m == -INFINITY ? 0.f : own.m;
-#pragma unroll
-    for (int i = 0; i < TL_INFLIGHT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) own.s += __expf(x[i][j] - ref);
+    const float ref = own.m == -INFINITY ? 0.f : -own.m;
+    const tl_pair ref2 = tl_two(ref, ref), scale2 = tl_two(TL_LOG2E, TL_LOG2E);
+    tl_pair sum2 = tl_two(own.s, 0.f);
 #pragma unroll
     for (int i = 0; i < TL_INFLIGHT; ++i) {
-      const int v = 4 * (p + i * THREADS) - row.off;
-      if (!by_key) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) before += x[i][j] > (v + j < t ? below : xt);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          before += p + i * THREADS < p1 && v + j >= 0 && v + j < vocab && tl_key(x[i][j], v + j) > mine;
-      }
+      const float2 a = tl_apart(tl_mul(tl_add(tl_two(f[i].x, f[i].y), ref2), scale2));
+      const float2 b = tl_apart(tl_mul(tl_add(tl_two(f[i].z, f[i].w), ref2), scale2));
+      sum2 = tl_add(sum2, tl_two(tl_exp2(a.x), tl_exp2(a.y)));
+      sum2 = tl_add(sum2, tl_two(tl_exp2(b.x), tl_exp2(b.y)));
     }
-  }
-
-  // the thread's largest key: the first logit equal to its maximum, in the pieces that brought it
-  // (without a maximum: the first -inf, wherever it stands, or its first NaN)
-  tl_key_t key = 0;
-  if (top > 0 && p0 + tid < p1) {
-    const tl_key_t lowest = tl_key(-INFINITY, 0x7fffffff);
-    for (int from = best_at; from < p1; from += TL_INFLIGHT * THREADS) {
+    const float2 sum = tl_apart(sum2);
+    own.s = sum.x + sum.y;
+    if (by_key) {
 #pragma unroll
       for (int i = 0; i < TL_INFLIGHT; ++i) {
-        const int p = from + i * THREADS;
-        if (p < p1) {
-          const float4 f = row.load(p);
-          const float x[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int v = 4 * p - row.off + j;
-            const tl_key_t k = v >= 0 && v < vocab ? tl_key(x[j], v) : 0;
-            if (k > key) key = k;
-          }
-        }
+        const int p = at + tid + i * THREADS, v = head + 4 * p;
+        if (p < p1)
+          before += (tl_key(f[i].x, v) > mine) + (tl_key(f[i].y, v + 1) > mine) +
+                    (tl_key(f[i].z, v + 2) > mine) + (tl_key(f[i].w, v + 3) > mine);
       }
-      if (key >= lowest) break;
+    } else if (m > below) {               // (most often nothing here stands before the token)
+#pragma unroll
+      for (int i = 0; i < TL_INFLIGHT; ++i) {
+        const int v = head + 4 * (at + tid + i * THREADS);
+        before += (f[i].x > (v < t ? below : xt)) + (f[i].y > (v + 1 < t ? below : xt)) +
+                  (f[i].z > (v + 2 < t ? below : xt)) + (f[i].w > (v + 3 < t ? below : xt));
+      }
     }
-  }
+  };
+  int at = p0;
+  for (; at + STEP <= p1; at += STEP) chunk(at, true);
+  if (at < p1) chunk(at, false);
 
   TlSum all = own;
 #pragma unroll
@@ -214,64 +238,122 @@ token_logprobs_kernel(float* __restrict__ logprob, int* __restrict__ rank, int* 
     s_sum[warp] = all;
     s_before[warp] = before;
   }
-  if (tid == 0) s_found = 0;
 
-  // joins the warps' sorted lists; warp 0 is left with the block's
-  auto join_lists = [&](tl_key_t mine_sorted, int lists) {
-    tl_key_t k = mine_sorted;
-    if (warp < lists) s_list[warp][lane] = k;
-    __syncthreads();
-    for (int half = lists / 2; half > 0; half >>= 1) {
-      if (warp < half) {
-        k = tl_merged(k, s_list[warp + half][31 - lane], lane);
-        s_list[warp][lane] = k;
-      }
-      __syncthreads();
-    }
-    return k;
-  };
-  tl_key_t best = 0;                        // warp 0: the block's alternatives, in order
   if (top > 0) {
-    join_lists(tl_sorted(key, lane), WARPS);
-    tl_key_t bound = s_list[0][top - 1];    // the top-th largest of the threads' maxima
+    const bool holds = p0 + tid < p1;
     const int rounds = (p1 - p0 + THREADS - 1) / THREADS;
-    int owners = 0;                         // threads whose maximum reaches it
-    for (int i = 0; i < top; ++i) owners += s_list[0][i] != 0;
-    const tl_key_t owner_key = s_list[0][lane];
-    __syncthreads();
-    // item q: piece q % rounds of owner q / rounds; owners are spread over the block
-    for (int from = 0; from < owners * rounds; from += TL_CAND / 4) {
-      const int to = min(owners * rounds, from + TL_CAND / 4);
-      for (int q0 = from + warp * 32; q0 < to; q0 += THREADS) {
-        const int q = q0 + lane;
-        const int o = min(q / rounds, TL_TOP - 1);
-        const tl_key_t ok = __shfl_sync(0xffffffffu, owner_key, o);
-        const int p = (int)(((unsigned)(tl_index(ok) + row.off) / 4 - p0) % THREADS) + p0 +
-                      (q % rounds) * THREADS;
-        if (q < to && p < p1) {
-          const float4 f = row.load(p);
-          const float x[4] = {f.x, f.y, f.z, f.w};
+    const int elements = 4 * (p1 - p0) + (part == 0 ? head + tail : 0);
+    // piece `round` of thread `who`, or one behind the block's
+    auto again = [&](int who, int round, tl_key_t bound) {
+      const int p = p0 + who + round * THREADS;
+      if (p >= p1) return;
+      const float4 f = row[p];
+      const float x[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int v = 4 * p - row.off + j;
-            if (v < 0 || v >= vocab) continue;
-            const tl_key_t k = tl_key(x[j], v);
-            if (k >= bound) s_cand[atomicAdd(&s_found, 1)] = k;
-          }
+      for (int j = 0; j < 4; ++j) {
+        const tl_key_t k = tl_key(x[j], head + 4 * p + j);
+        if (k >= bound) {
+          const int i = atomicAdd(&s_found, 1);
+          if (i < TL_CAND) s_cand[i] = k;
+        }
+      }
+    };
+    auto again_edge = [&](tl_key_t bound) {
+      if (edge < 0) return;
+      const tl_key_t k = tl_key(base[edge], edge);
+      if (k >= bound) {
+        const int i = atomicAdd(&s_found, 1);
+        if (i < TL_CAND) s_cand[i] = k;
+      }
+    };
+    const uint32_t own_order = holds ? tl_order(m_pieces) : 0u;
+    uint32_t g = own_order;
+#pragma unroll
+    for (int o = THREADS / TL_GROUPS / 2; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+    if (tid % (THREADS / TL_GROUPS) == 0) s_group[tid / (THREADS / TL_GROUPS)] = g;
+    if (tid == 0) s_owners = s_found = 0;
+    if (tid < TL_TOP) s_top[tid] = 0;
+    __syncthreads();
+    uint32_t reach = s_group[lane];
+    int larger = 0;
+#pragma unroll
+    for (int i = 0; i < TL_GROUPS; i += 4) {
+      const uint4 o = *(const uint4*)&s_group[i];
+      larger += (o.x >= reach) + (o.y >= reach) + (o.z >= reach) + (o.w >= reach);
+    }
+    reach = __reduce_max_sync(0xffffffffu, larger >= top ? reach : 0u);
+    if (holds && own_order >= reach) s_owner[atomicAdd(&s_owners, 1)] = (uint16_t)tid;
+    __syncthreads();
+    const int owners = s_owners;
+    bool done = owners * 4 <= TL_CAND;    // else more is equal than a list takes, or nearly so
+    if (done) {
+      for (int q = tid; q < owners * rounds; q += THREADS)
+        again(s_owner[q / rounds], q % rounds, (tl_key_t)reach << 32);
+      again_edge((tl_key_t)reach << 32);
+      __syncthreads();
+      const int found = s_found;
+      done = found <= TL_CAND && found >= min(top, elements);
+      if (done) {
+        for (int i = tid; i < found; i += THREADS) {
+          const tl_key_t k = s_cand[i];
+          int place = 0;
+          for (int j = 0; j < found; ++j) place += s_cand[j] > k;
+          if (place < TL_TOP) s_top[place] = k;
         }
       }
       __syncthreads();
-      const int found = s_found;
-      if (warp == 0) {
-        for (int i = 0; i < found; i += 32)
-          best = tl_merged(best, __shfl_sync(0xffffffffu, tl_sorted(i + lane < found ? s_cand[i + lane] : 0, lane),
-                                             31 - lane), lane);
-        s_list[0][lane] = best;
-        if (lane == 0) s_found = 0;
+    }
+    if (!done) {
+      // the threads' largest keys in order: those of the first `top` hold what is looked for
+      tl_key_t key = 0;
+      for (int p = p0 + tid; p < p1; p += THREADS) {
+        const float4 f = row[p];
+        const float x[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const tl_key_t k = tl_key(x[j], head + 4 * p + j);
+          if (k > key) key = k;
+        }
       }
+      tl_key_t k = tl_sorted(key, lane);
+      s_list[warp][lane] = k;
+      if (tid == 0) s_found = 0;
       __syncthreads();
-      const tl_key_t reached = s_list[0][top - 1];
-      if (reached > bound) bound = reached;
+      for (int half = WARPS / 2; half > 0; half >>= 1) {
+        if (warp < half) {
+          k = tl_merged(k, s_list[warp + half][31 - lane], lane);
+          s_list[warp][lane] = k;
+        }
+        __syncthreads();
+      }
+      tl_key_t bound = s_list[0][top - 1];
+      const int who = (int)((unsigned)(tl_index(s_list[0][lane]) - head) / 4 - p0) % THREADS;
+      const int last = __popc(__ballot_sync(0xffffffffu, lane < top && s_list[0][lane] != 0));
+      __syncthreads();
+      tl_key_t best = 0;                  // warp 0: what has been found so far, in order
+      again_edge(bound);
+      constexpr int ITEMS = (TL_CAND - 8) / 4;
+      for (int from = 0; from == 0 || from < last * rounds; from += ITEMS) {
+        const int to = min(last * rounds, from + ITEMS);
+        for (int q0 = from + warp * 32; q0 < to; q0 += THREADS) {
+          const int q = q0 + lane, thread = __shfl_sync(0xffffffffu, who, min(q / rounds, 31));
+          if (q < to) again(thread, q % rounds, bound);
+        }
+        __syncthreads();
+        const int found = s_found;
+        __syncthreads();
+        if (warp == 0) {
+          for (int i = 0; i < found; i += 32) {
+            const tl_key_t next = tl_sorted(i + lane < found ? s_cand[i + lane] : 0, lane);
+            best = tl_merged(best, __shfl_sync(0xffffffffu, next, 31 - lane), lane);
+          }
+          s_top[lane] = best;
+          if (lane == 0) s_found = 0;
+        }
+        __syncthreads();
+        if (s_top[top - 1] > bound) bound = s_top[top - 1];
+        __syncthreads();
+      }
     }
   }
   __syncthreads();
@@ -282,23 +364,20 @@ token_logprobs_kernel(float* __restrict__ logprob, int* __restrict__ rank, int* 
     for (int o = 16; o > 0; o >>= 1)
       all = tl_join(all, TlSum{__shfl_xor_sync(0xffffffffu, all.m, o), __shfl_xor_sync(0xffffffffu, all.s, o)});
     before = __reduce_add_sync(0xffffffffu, before);
+    if (lane == 0) {
+      s_block = all;
+      s_block_before = before;
+    }
   }
   if constexpr (BLOCKS > 1) {
-    if (warp == 0) {
-      s_list[0][lane] = best;
-      if (lane == 0) {
-        s_block = all;
-        s_block_before = before;
-      }
-    }
     tl_cluster_sync();
     if (part == 0) {
-      if (top > 0) {
-        const tl_key_t k = warp < BLOCKS ? tl_remote(&s_list[0][lane], warp) : 0;
-        __syncthreads();                    // (this block's own list is read before it is replaced)
-        best = join_lists(k, BLOCKS);
+      tl_key_t k = 0;
+      if (tid < BLOCKS * top) {
+        k = tl_remote(&s_top[tid % top], tid / top);
+        s_cand[tid] = k;
       }
-      if (warp == 0) {
+      if (warp == WARPS - 1) {            // (a warp that has no list to fetch where there are others)
         all = lane < BLOCKS ? TlSum{tl_remote(&s_block.m, lane), tl_remote(&s_block.s, lane)}
                             : TlSum{-INFINITY, 0.f};
         before = lane < BLOCKS ? tl_remote(&s_block_before, lane) : 0;
@@ -307,21 +386,36 @@ token_logprobs_kernel(float* __restrict__ logprob, int* __restrict__ rank, int* 
           all = tl_join(all, TlSum{__shfl_xor_sync(0xffffffffu, all.m, o), __shfl_xor_sync(0xffffffffu, all.s, o)});
         before = __reduce_add_sync(0xffffffffu, before);
       }
+      __syncthreads();                    // (the block's own share has been read as well)
+      if (warp == WARPS - 1 && lane == 0) {
+        s_block = all;
+        s_block_before = before;
+      }
+      if (k != 0) {
+        int place = 0;
+        for (int j = 0; j < BLOCKS * top; ++j) place += s_cand[j] > k;
+        if (place < top) s_list[0][place] = k;
+      }
     }
-    tl_cluster_sync();                      // the others stay until their memory has been read
+    tl_cluster_sync();                    // the others stay until their memory has been read
+    if (part != 0) return;
+  } else {
+    __syncthreads();
   }
-  if (part != 0 || warp != 0) return;
-  const float log_sum = logf(all.s);
+  const tl_key_t* found = BLOCKS > 1 ? s_list[0] : s_top;
+  const TlSum total = s_block;
+  const float log_sum = logf(total.s);
   // (without a maximum the sum is 0, or NaN where a NaN was: -inf then, or NaN)
-  auto lp = [&](float x) { return all.m == -INFINITY ? log_sum : (x - all.m) - log_sum; };
-  if (lane == 0) {
+  auto lp = [&](float x) { return total.m == -INFINITY ? log_sum : (x - total.m) - log_sum; };
+  if (tid == 0) {
     logprob[w] = given ? lp(xt) : __int_as_float(0x7fffffff);
-    rank[w] = given ? before : -1;
+    rank[w] = given ? s_block_before : -1;
     if (!given && t != -1) atomicOr(status, HS_STATUS_BAD_TOKEN);
   }
-  if (lane < top) {
-    top_ids[(size_t)w * top + lane] = tl_index(best);
-    top_logprobs[(size_t)w * top + lane] = lp(tl_value(best));
+  if (tid < top) {
+    const tl_key_t k = found[tid];
+    top_ids[(size_t)w * top + tid] = tl_index(k);
+    top_logprobs[(size_t)w * top + tid] = lp(tl_value(k));
   }
 }
 
@@ -367,7 +461,12 @@ HS_EXPORT int hs_token_logprobs(float* logprob, int* rank, int* top_ids, float* 
   if (rows <= 0) return HS_OK;
   if (rows > (1 << 27) || vocab > 0x7ffffff0) return HS_ERR_UNSUPPORTED;
   cudaStream_t st = (cudaStream_t)stream;
-  const int blocks = vocab <= 4096 ? 1 : rows <= 74 ? 8 : rows <= 148 ? 4 : rows <= 296 ? 2 : 1;
+  // A row over 8, 4 or 2 blocks of 512 threads while that gives every SM two blocks or fewer, and
+  // only where it is long: us in a graph, one block against the choice, with 20 alternatives:
+  // 1 x 50,257 8.3 and 7.0, 64 x 50,257 8.8 and 9.1 (18.5 and 16.4 with the logits out of the L2),
+  // 128 x 50,257 11.7 and 10.6, 32 x 131,072 13.7 and 10.0; 32 x 16,384 5.6 and over 2 blocks 6.6.
+  // Short rows take half the threads (128 x 4,096: 4.8, with 512 threads 6.1).
+  const int blocks = vocab <= 24576 ? 1 : rows <= 37 ? 8 : rows <= 74 ? 4 : rows <= 148 ? 2 : 1;
   cudaError_t e;
 #define TL_GO(THREADS, BLOCKS)                                                                      \
   e = hs::token_logprobs<THREADS, BLOCKS>(logprob, rank, top_ids, top_logprobs, top, logits, tokens, \
@@ -375,7 +474,7 @@ HS_EXPORT int hs_token_logprobs(float* logprob, int* rank, int* top_ids, float* 
   if (blocks == 8) TL_GO(512, 8);
   else if (blocks == 4) TL_GO(512, 4);
   else if (blocks == 2) TL_GO(512, 2);
-  else if (vocab <= 4096) TL_GO(256, 1);
+  else if (vocab <= 8192) TL_GO(256, 1);
   else TL_GO(512, 1);
 #undef TL_GO
   return e == cudaSuccess ? HS_OK : (int)e;
