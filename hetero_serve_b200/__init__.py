@@ -8,8 +8,9 @@ a continuous-batching scheduler, device-side sampling, and hand-written CUDA ker
 
 from . import architectures  # noqa: F401
 from .config import EngineConfig, preset
-from .engine import LLMEngine, Request, RequestRecord, Runner, StepEntry
+from .engine import LLMEngine, Request, RequestRecord, Runner, StepEntry, TokenLogprobs
+from .sampling import LogitRules, OneOf
 
 __version__ = "0.1.0"
-__all__ = ["EngineConfig", "LLMEngine", "Request", "RequestRecord", "Runner",
-           "StepEntry", "preset"]
+__all__ = ["EngineConfig", "LLMEngine", "LogitRules", "OneOf", "Request", "RequestRecord", "Runner",
+           "StepEntry", "TokenLogprobs", "preset"]

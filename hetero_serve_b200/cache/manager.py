@@ -165,6 +165,41 @@ class PagePool:
     def refcount(self, page: int) -> int:
         return self._ref[page]
 
+    def share(self, page: int) -> None:
+        """One more holder of a page somebody holds, published or not (a fork)."""
+        if self._ref[page] <= 0:
+            raise CacheError(f"page {page} is not held: it cannot be shared")
+        self._ref[page] += 1
+
+    # another size ----------------------------------------------------------
+    def num_held(self) -> int:
+        return sum(1 for r in self._ref if r > 0)
+
+    def resize(self, num_pages: int) -> dict[int, int]:
+        """Renumber the pages for a pool of ``num_pages``: held ones, and as many of the published
+        ones nobody holds as fit (the oldest are evicted first), get the lowest numbers in their
+        order.  Returns old number -> new number, or raises :class:`OutOfPages` with nothing
+        changed."""
+        held = [p for p in range(self.num_pages) if self._ref[p] > 0]
+        if num_pages <= 0 or len(held) > num_pages:
+            raise OutOfPages(f"{len(held)} pages are held: they do not fit {num_pages}")
+        drop = max(0, len(held) + len(self._evictable) - num_pages)
+        for _ in range(drop):
+            h, _none = self._evictable.popitem(last=False)
+            del self._page_to_hash[self._hash_to_page.pop(h)]
+            self.evictions += 1
+        stay = sorted(held + [self._hash_to_page[h] for h in self._evictable])
+        moved = {old: new for new, old in enumerate(stay)}
+        ref = [0] * num_pages
+        for old in held:
+            ref[moved[old]] = self._ref[old]
+        self._ref = ref
+        self._hash_to_page = {h: moved[p] for h, p in self._hash_to_page.items()}
+        self._page_to_hash = {p: h for h, p in self._hash_to_page.items()}
+        self._free = list(range(num_pages - 1, len(stay) - 1, -1))
+        self.num_pages = num_pages
+        return moved
+
     def check(self, held: dict[int, int]) -> None:
         """Invariant: every page is exactly one of free / evictable / held, and the count of
         a held page equals the number of tables that list it (``held``: page → holders)."""
@@ -301,6 +336,59 @@ class CacheManager:
         if self.on_open is not None:
             self.on_open(req.slot)
         return Opened(req.slot, req.cached_tokens)
+
+    def fork(self, req_id, child_id) -> list[list[tuple[int, int, int]]]:
+        """Start ``child_id`` as a copy of ``req_id``: full pages are shared, a partly filled last
+        page gets a page of its own.  Returns per group what has to be copied, (from page, to
+        page, filled rows); the state slot is the child's own.  Raises :class:`OutOfPages` with
+        nothing changed.  (A full page is never written again, so sharing it is sound in windowed,
+        chunked and companion groups too, published or not.)"""
+        req = self._get(req_id)
+        if child_id in self._requests:
+            raise CacheError(f"request {child_id!r} is already open")
+        if not self._free_slots:
+            raise OutOfPages("no state slot free")
+        filled = [divmod(req.length // g.stride, self.page_size) for g in self.groups]
+        own = [rows > 0 and full < len(t) and t[full] >= 0
+               for (full, rows), t in zip(filled, req.tables)]
+        for need, pool in zip(own, self.pools):
+            if need and pool.num_free < 1:
+                raise OutOfPages("1 page wanted, 0 obtainable")
+        child = _Request(slot=self._free_slots.pop(), length=req.length,
+                         first_live=list(req.first_live), cached_tokens=req.length,
+                         published=req.published)
+        copies: list[list[tuple[int, int, int]]] = []
+        for pool, table, (full, rows), need in zip(self.pools, req.tables, filled, own):
+            shared = list(table[:full])
+            for page in shared:
+                if page >= 0:
+                    pool.share(page)
+            copies.append([])
+            if need:
+                page = pool.take(1)[0]
+                copies[-1].append((table[full], page, rows))
+                shared.append(page)
+            elif rows > 0 and full < len(table):
+                shared.append(table[full])                 # given back already
+            child.tables.append(shared)
+        self._requests[child_id] = child
+        if self.on_open is not None:
+            self.on_open(child.slot)
+        return copies
+
+    def resize(self, num_pages: Sequence[int]) -> list[dict[int, int]]:
+        """Give every group's pool another size; returns per group old page -> new page (see
+        :meth:`PagePool.resize`).  Raises :class:`OutOfPages` with nothing changed."""
+        if len(num_pages) != len(self.pools):
+            raise ValueError(f"{len(num_pages)} sizes for {len(self.pools)} pools")
+        for pool, n in zip(self.pools, num_pages):
+            if n <= 0 or pool.num_held() > n:
+                raise OutOfPages(f"{pool.num_held()} pages are held: they do not fit {n}")
+        moves = [pool.resize(n) for pool, n in zip(self.pools, num_pages)]
+        for req in self._requests.values():
+            for gi, moved in enumerate(moves):
+                req.tables[gi] = [moved[p] if p >= 0 else p for p in req.tables[gi]]
+        return moves
 
     def rematch(self, req_id, token_ids: Sequence[int]) -> int:
         """Try the prefix match again for a request that has computed nothing since it was

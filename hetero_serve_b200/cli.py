@@ -55,6 +55,15 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--top-k", dest="top_k", type=int, default=0)
     ap.add_argument("--sample-seed", dest="sample_seed", type=int, default=None,
                     help="seed of the sampling draws (request i uses seed + i); default: --seed")
+    ap.add_argument("--samples", type=int, default=1,
+                    help="answers to each prompt (they share its pages; answer i adds i to the seed)")
+    ap.add_argument("--repetition-penalty", dest="repetition_penalty", type=float, default=1.0)
+    ap.add_argument("--presence-penalty", dest="presence_penalty", type=float, default=0.0)
+    ap.add_argument("--frequency-penalty", dest="frequency_penalty", type=float, default=0.0)
+    ap.add_argument("--logit-bias", dest="logit_bias", action="append", default=[],
+                    metavar="ID:VALUE", help="added to a token's logit (-inf: never); repeatable")
+    ap.add_argument("--logprobs", type=int, default=None,
+                    help="score every generated token, with this many alternatives (--json shows them)")
     ap.add_argument("--no-eos-stop", dest="stop_at_eos", action="store_false")
     ap.add_argument("--json", action="store_true", help="one JSON object per request")
     return ap
@@ -100,15 +109,20 @@ def main(argv=None) -> int:
 
     sample_seed = args.seed if args.sample_seed is None else args.sample_seed
 
+    bias = {int(t): float(v) for t, v in (b.split(":") for b in args.logit_bias)}
+
     def req(p, i=0):
         return Request(p, args.max_new_tokens, args.temperature, args.top_k, sample_seed + i,
-                       args.stop_at_eos)
+                       args.stop_at_eos, repetition_penalty=args.repetition_penalty,
+                       presence_penalty=args.presence_penalty,
+                       frequency_penalty=args.frequency_penalty, logit_bias=bias,
+                       logprobs=args.logprobs, samples=args.samples)
 
     t0 = time.perf_counter()
     if prompts:
         seqs = [engine.submit_nowait(req(p, i)) for i, p in enumerate(prompts)]
         records = engine.run_until_done()
-        order = {s.req_id: i for i, s in enumerate(seqs)}
+        order = {a.req_id: (i, j) for i, s in enumerate(seqs) for j, a in enumerate([s, *s.siblings])}
         records.sort(key=lambda r: order[r.req_id])
         for r in records:
             _report(r, args.json)

@@ -9,7 +9,7 @@
 
 namespace hs {
 
-constexpr int PC_THREADS = 256;
+constexpr int PC_THREADS = 256, PC_INFLIGHT = 4;
 constexpr int PC_FEW = 32, PC_MANY = 1024;     // pairs a launch takes
 
 template <int PAIRS>
@@ -18,21 +18,32 @@ struct PageList {
   short rows[PAIRS];
 };
 
+// One block a pair, an entry and a share of the page's filled rows, counted in pieces of V.
 template <typename V, int PAIRS>
 __global__ void __launch_bounds__(PC_THREADS)
 copy_pages_kernel(V* dst, const V* src, long long dst_pages, long long src_pages, int tiles,
-                  int page_rows, int row_vecs, const __grid_constant__ PageList<PAIRS> list) {
+                  int page_rows, int row_vecs, int share, const __grid_constant__ PageList<PAIRS> list) {
   pdl_trigger();
   pdl_wait();
   const int i = blockIdx.x, e = blockIdx.y;
-  const int rows = list.rows[i];
-  const int tile_vecs = page_rows * row_vecs, live = rows * row_vecs;
+  const int tile_vecs = page_rows * row_vecs, live = list.rows[i] * row_vecs;
+  const bool whole = live == tile_vecs;
   const size_t page_vecs = (size_t)tiles * tile_vecs;
   V* to = dst + (e * dst_pages + list.dst[i]) * page_vecs;
   const V* from = src + (e * src_pages + list.src[i]) * page_vecs;
-  for (int j = threadIdx.x; j < tiles * live; j += PC_THREADS) {
-    const int at = j / live * tile_vecs + j % live;
-    to[at] = from[at];
+  const int j0 = blockIdx.z * share, j1 = min(tiles * live, j0 + share);
+  for (int j = j0 + threadIdx.x; j < j1; j += PC_INFLIGHT * PC_THREADS) {
+    V x[PC_INFLIGHT];
+    int at[PC_INFLIGHT];
+#pragma unroll
+    for (int k = 0; k < PC_INFLIGHT; ++k) {
+      const int q = j + k * PC_THREADS;
+      at[k] = whole ? q : q / live * tile_vecs + q % live;
+      if (q < j1) x[k] = from[at[k]];
+    }
+#pragma unroll
+    for (int k = 0; k < PC_INFLIGHT; ++k)
+      if (j + k * PC_THREADS < j1) to[at[k]] = x[k];
   }
 }
 
@@ -48,10 +59,17 @@ cudaError_t copy_pages(void* dst, const void* src, int n, const int* dst_list, c
       list.src[i] = src_list[from + i];
       list.rows[i] = (short)(rows ? rows[from + i] : page_rows);
     }
-    const cudaError_t e = hs_launch(copy_pages_kernel<V, PAIRS>, dim3(count, entries), dim3(PC_THREADS), 0,
-                                    stream, hs_pdl_enabled(), (V*)dst, (const V*)src,
-                                    (long long)dst_pages, (long long)src_pages, tiles, page_rows,
-                                    (int)(row_bytes / sizeof(V)), list);
+    // shares of a page of four rounds of a block's loads or more, two of them at least an SM
+    const int row_vecs = (int)(row_bytes / sizeof(V)), page_vecs = tiles * page_rows * row_vecs;
+    const int round = PC_INFLIGHT * PC_THREADS;
+    int share = 4 * round;
+    while (share > round && (long long)count * entries * ((page_vecs + share - 1) / share) < 2 * 148) share /= 2;
+    const int shares = (page_vecs + share - 1) / share;
+    if (shares > 65535) return cudaErrorInvalidValue;
+    const cudaError_t e = hs_launch(copy_pages_kernel<V, PAIRS>, dim3(count, entries, shares),
+                                    dim3(PC_THREADS), 0, stream, hs_pdl_enabled(), (V*)dst,
+                                    (const V*)src, (long long)dst_pages, (long long)src_pages, tiles,
+                                    page_rows, row_vecs, share, list);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -67,7 +85,7 @@ HS_EXPORT int hs_copy_pages(void* dst, const void* src, int n, const int* dst_li
   if (n <= 0) return HS_OK;
   if (!dst || !src || !dst_list || !src_list) return HS_ERR_ARGUMENT;
   if (entries <= 0 || entries > 65535 || tiles <= 0 || page_rows <= 0 || page_rows > 32767 ||
-      row_bytes <= 0 || row_bytes % 2 || (long long)tiles * page_rows * row_bytes > 0x7fffffffLL)
+      row_bytes <= 0 || row_bytes % 2 || (long long)tiles * page_rows * row_bytes > (1LL << 27))
     return HS_ERR_UNSUPPORTED;
   for (int i = 0; i < n; ++i)
     if (dst_list[i] < 0 || dst_list[i] >= dst_pages || src_list[i] < 0 || src_list[i] >= src_pages ||

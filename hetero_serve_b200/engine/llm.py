@@ -3,6 +3,8 @@
     engine = LLMEngine("path/to/model", dtype="bfloat16", num_blocks=512)
     record = engine.submit(Request(prompt_ids=[...], max_new_tokens=32))
     outputs = engine.generate([[...], [...]], max_new_tokens=16, temperature=0.8, seed=1)
+    answers = engine.submit_samples(Request(prompt_ids=[...], samples=8, temperature=0.8, logprobs=0))
+    scores = engine.score([...], alternatives=5)
 
 ``Request`` and ``RequestRecord`` carry the reference's names
 (heteroserve/sched/router.py:36-44, heteroserve/metrics.py:31-68); ``submit`` is the
@@ -14,16 +16,21 @@ continuous-batching loop for callers that feed requests while others run.
 from __future__ import annotations
 
 import tempfile
+import itertools
 from dataclasses import replace
 from pathlib import Path
 from typing import Sequence
+
+import torch
 
 from ..config import EngineConfig, preset
 from ..weights import write_model_dir
 from .loading import TORCH_DTYPES, load_model
 from .metrics import RequestRecord, summarise
 from .scheduler import Request, Scheduler, SequenceState
-from .step import Runner, StepEntry
+from .step import Runner, StepEntry, TokenLogprobs
+
+_scored = itertools.count()
 
 
 class LLMEngine:
@@ -46,7 +53,7 @@ class LLMEngine:
             self.runner.manager, self._run_step, max_batch=cfg.max_batch,
             max_prefill_tokens=cfg.max_prefill_tokens, max_ctx=max_ctx,
             eos_token_id=spec.eos_token_id, policy=cfg.policy, vocab_size=spec.vocab_size,
-            pipeline=cfg.pipeline)
+            pipeline=cfg.pipeline, fork_fn=self.runner.fork)
         self._tmp = None
 
     # -- construction --------------------------------------------------------------
@@ -101,12 +108,62 @@ class LLMEngine:
             self.step()
         return RequestRecord.of(seq)
 
+    def submit_samples(self, request: Request) -> list[RequestRecord]:
+        """Run until every answer to this request's prompt has finished (``request.samples`` of
+        them, in the order of their seeds; others in flight advance too)."""
+        seq = self.submit_nowait(request)
+        answers = [seq, *seq.siblings]
+        while any(s.state != "done" for s in answers):
+            self.step()
+        return [RequestRecord.of(s) for s in answers]
+
+    def score(self, token_ids: Sequence[int], alternatives: int = 0) -> list[TokenLogprobs]:
+        """Score given text: the log-probability and rank of every token but the first behind the
+        ones before it, with the likeliest ``alternatives`` at its place.  Runs beside live
+        requests, in portions of the engine's token budget, and needs a state slot and pages for
+        the text meanwhile (:class:`OutOfPages` otherwise)."""
+        runner, text = self.runner, [int(t) for t in token_ids]
+        name, out = ("score", next(_scored)), []
+        with runner._on_device():
+            runner.open(name)
+            try:
+                for at in range(0, len(text) - 1, self.config.max_prefill_tokens):
+                    part = text[at:min(at + self.config.max_prefill_tokens, len(text) - 1)]
+                    res = runner.step([StepEntry(name, part, want=range(len(part)))])
+                    out += self._scores(res.logits, text[at + 1:at + 1 + len(part)], alternatives)
+            finally:
+                runner.close(name)
+        return out
+
+    def _scores(self, logits, tokens, alternatives) -> list[TokenLogprobs]:
+        n, dev = len(tokens), logits.device
+        given = torch.tensor(tokens, dtype=torch.int32, device=dev)
+        logprob = torch.empty(n, device=dev)
+        rank = torch.empty(n, dtype=torch.int32, device=dev)
+        ids = torch.empty(n, alternatives, dtype=torch.int32, device=dev)
+        lps = torch.empty(n, alternatives, device=dev)
+        self.runner.ops.token_logprobs(logprob, rank, logits, given,
+                                       *((ids, lps) if alternatives else ()))
+        return [TokenLogprobs(lp, r, list(zip(i, p))) for lp, r, i, p in
+                zip(logprob.tolist(), rank.tolist(), ids.tolist(), lps.tolist())]
+
+    def resize_cache(self, num_blocks: int) -> None:
+        """Make the cache smaller or larger while requests live: their pages move to the lowest
+        numbers of pools of the new size, published prefixes as far as they fit.  Raises
+        :class:`OutOfPages`, with nothing changed, where the live requests' pages do not fit.
+        The longest request the engine takes stays what it was."""
+        self.runner.resize_cache(num_blocks)
+        self.config = replace(self.config, num_blocks=num_blocks)
+
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 32,
                  temperature: float = 0.0, top_k: int = 0, seed: int = 0,
-                 stop_at_eos: bool = True) -> list[list[int]]:
-        """Generate for several prompts at once; returns the new token ids of each."""
+                 stop_at_eos: bool = True, **options) -> list[list[int]]:
+        """Generate for several prompts at once; returns the new token ids of each.  ``options``
+        are further fields of :class:`Request` (penalties, ``logit_bias``; one answer a prompt)."""
+        if options.get("samples", 1) != 1:
+            raise ValueError("generate gives one answer a prompt: see submit_samples")
         seqs = [self.submit_nowait(Request(list(p), max_new_tokens, temperature, top_k,
-                                           seed + i, stop_at_eos))
+                                           seed + i, stop_at_eos, **options))
                 for i, p in enumerate(prompts)]
         self.run_until_done()
         return [list(s.output_ids) for s in seqs]

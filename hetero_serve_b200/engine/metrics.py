@@ -47,6 +47,13 @@ class RequestRecord:
     t_admit: float = 0.0
     t_first_token: float = 0.0
     t_done: float = 0.0
+    # scores of the generated tokens (``TokenLogprobs``), where the request asked for them
+    scores: list = field(default_factory=list)
+
+    @property
+    def cumulative_logprob(self) -> float:
+        """Log-probability of the whole answer (NaN where no scores were asked for)."""
+        return sum(s.logprob for s in self.scores) if self.scores else NAN
 
     @property
     def ttft(self) -> float:
@@ -73,6 +80,11 @@ class RequestRecord:
             "prefill_tokens_computed", "preemptions", "finish_reason")}
         out.update(ttft=round(self.ttft, 5), tpot=round(self.tpot, 6), e2e=round(self.e2e, 5),
                    cache_hit_rate=round(self.cache_hit_rate, 4), output_ids=list(self.output_ids))
+        if self.scores:
+            out.update(cumulative_logprob=round(self.cumulative_logprob, 5),
+                       logprobs=[round(s.logprob, 5) for s in self.scores],
+                       ranks=[s.rank for s in self.scores],
+                       top_logprobs=[[(t, round(lp, 5)) for t, lp in s.top] for s in self.scores])
         return out
 
     @classmethod
@@ -84,7 +96,7 @@ class RequestRecord:
                    prefill_tokens_computed=seq.prefill_tokens_computed,
                    preemptions=seq.preemptions, finish_reason=seq.finish_reason,
                    output_ids=list(seq.output_ids), t_submit=seq.t_submit, t_admit=seq.t_admit,
-                   t_first_token=seq.t_first_token, t_done=seq.t_done)
+                   t_first_token=seq.t_first_token, t_done=seq.t_done, scores=list(seq.scores))
 
 
 def summarise(records: list[RequestRecord], wall_s: float) -> dict:

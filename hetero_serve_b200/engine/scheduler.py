@@ -43,7 +43,14 @@ out (its end is known by counting); an end-of-sequence token is seen one step la
 request's part in the step launched meanwhile is discarded (its pages were still its own when
 that step was launched, and whoever gets them next is ordered behind it on the stream);
 preemption first waits for the tokens in flight, since a preempted request is prefilled again
-over all of its tokens.
+over all of its tokens; a request whose grammar has to see the token before it can say what may
+follow sits out the steps in which its token is in flight.
+
+Several answers to one prompt (``Request.samples``).  The prompt is prefilled once, all but its
+last token; then the request is forked (``fork_fn``): its full pages are shared, its last page and
+state copied, and every sample decodes on its own, the last prompt token first, with a seed of its
+own (``seed + i``).  A sample for which no page or slot can be had queues as a request of its own
+at the front, and finds the prompt's pages by prefix reuse.
 """
 
 from __future__ import annotations
@@ -51,10 +58,12 @@ from __future__ import annotations
 import itertools
 import time
 from collections import deque
-from dataclasses import dataclass, field
-from typing import Callable, Hashable, Sequence
+from dataclasses import dataclass, field, replace
+from typing import Callable, Hashable, Mapping, Sequence
 
 from ..cache import CacheManager, OutOfPages
+from ..kernels.ops import MAX_ALTERNATIVES
+from ..sampling import LogitRules, mask_words
 from .step import FROM_DEVICE, StepEntry
 
 
@@ -83,6 +92,18 @@ class Request:
     seed: int = 0
     stop_at_eos: bool = True
     req_id: Hashable = field(default_factory=lambda: f"req-{next(_ids)}")
+    # what may be said (see ``sampling.rules``)
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: Mapping[int, float] | None = None
+    grammar: object | None = None       # ``allowed(output_ids)``; a grammar answers for one request
+    logprobs: int | None = None         # scores of every token, with this many alternatives
+    samples: int = 1                    # answers to the prompt; answer i draws with seed + i
+
+    def rules(self) -> LogitRules:
+        return LogitRules(float(self.repetition_penalty), float(self.presence_penalty),
+                          float(self.frequency_penalty), dict(self.logit_bias or {}))
 
 
 @dataclass
@@ -99,6 +120,12 @@ class SequenceState:
     preemptions: int = 0
     finish_reason: str = ""
     pending: int = 0                    # tokens sampled for it that the host has not read yet
+    rules: LogitRules | None = None     # None: none that change anything
+    recorded: bool = False              # its tokens are on the device, for penalties
+    scores: list = field(default_factory=list)      # TokenLogprobs of its tokens, if asked for
+    # the other answers to its prompt, while they wait for it to be prefilled, and once forked
+    to_fork: list["SequenceState"] = field(default_factory=list)
+    siblings: list["SequenceState"] = field(default_factory=list)
     t_submit: float = 0.0
     t_admit: float = 0.0
     t_first_token: float = 0.0
@@ -114,9 +141,10 @@ class SequenceState:
 
     @property
     def prefill_target(self) -> int:
-        """How far prefill must reach before decoding takes over (worker.py:79-83)."""
+        """How far prefill must reach before decoding takes over (worker.py:79-83): the last
+        token is decoding's where it has been generated, or is fed by every sample."""
         n = len(self.request.prompt_ids) + len(self.output_ids)
-        return n - 1 if self.output_ids else n
+        return n - 1 if self.output_ids or self.request.samples > 1 else n
 
 
 @dataclass
@@ -152,7 +180,8 @@ class Scheduler:
                  *, max_batch: int, max_prefill_tokens: int, max_ctx: int,
                  eos_token_id: int | None, policy: str = "prefill_first",
                  vocab_size: int | None = None, clock: Callable[[], float] = time.perf_counter,
-                 pipeline: bool = False):
+                 pipeline: bool = False,
+                 fork_fn: Callable[[Hashable, Hashable], object] | None = None):
         if policy not in ("prefill_first", "mixed"):
             raise ValueError(f"unknown policy {policy!r}")
         self.manager = manager
@@ -169,6 +198,7 @@ class Scheduler:
         self.finished: list[SequenceState] = []
         self.stats = SchedulerStats()
         self.pipeline = bool(pipeline)
+        self.fork_fn = fork_fn or manager.fork
         self._inflight: tuple[list[Planned], object] | None = None   # launched, tokens unread
         self._late_done: list[SequenceState] = []     # finished while a plan was being made
 
@@ -191,7 +221,32 @@ class Scheduler:
                 raise RequestRefused(
                     f"the prompt needs {self.manager.pages_for(n + 1, gi)} pages, the pool has "
                     f"{pool.num_pages}")
-        seq = SequenceState(request=request, t_submit=self.clock())
+        try:
+            rules = request.rules()
+            rules.check(self.vocab_size)
+        except (TypeError, ValueError, OverflowError) as exc:
+            raise RequestRefused(str(exc)) from None
+        if request.grammar is not None and not callable(getattr(request.grammar, "allowed", None)):
+            raise RequestRefused("a grammar needs a method allowed(output_ids)")
+        if request.grammar is not None and self.vocab_size is None:
+            raise RequestRefused("a grammar needs a vocabulary size")
+        most = MAX_ALTERNATIVES if self.vocab_size is None else min(MAX_ALTERNATIVES, self.vocab_size)
+        if request.logprobs is not None and not 0 <= request.logprobs <= most:
+            raise RequestRefused(f"logprobs={request.logprobs}: between 0 and {most} alternatives")
+        if request.samples < 1:
+            raise RequestRefused(f"samples={request.samples}: at least one answer")
+        known = {s.req_id for s in [*self.waiting, *self.active]}
+        known |= {s.req_id for q in [*self.waiting, *self.active] for s in q.to_fork}
+        now = self.clock()
+        state = lambda r: SequenceState(request=r, t_submit=now,              # noqa: E731
+                                        rules=None if rules.neutral else rules)
+        seq = state(request)
+        for i in range(1, request.samples):
+            seq.siblings.append(state(replace(request, seed=request.seed + i, samples=1,
+                                              req_id=f"{request.req_id}#{i}")))
+        if request.samples > 1 and known & {s.req_id for s in [seq, *seq.siblings]}:
+            raise RequestRefused(f"request {request.req_id!r} is known already")
+        seq.to_fork = list(seq.siblings)
         self.waiting.append(seq)
         return seq
 
@@ -226,7 +281,31 @@ class Scheduler:
                 seq.t_admit = self.clock()
             self.stats.tokens_saved_by_cache += seq.n_kv
             seq.state = SeqState.PREFILL if seq.n_kv < target else SeqState.RUNNING
+            seq.recorded = False
             self.active.append(seq)
+            if seq.state == SeqState.RUNNING:
+                self._fork_samples(seq)
+
+    def _fork_samples(self, seq: SequenceState) -> None:
+        """The prompt is resident: start the other answers to it."""
+        at = self.active.index(seq) + 1
+        queued: list[SequenceState] = []
+        for other in seq.to_fork:
+            try:
+                if queued:
+                    raise OutOfPages("an earlier answer waits")
+                self.fork_fn(seq.req_id, other.req_id)
+            except OutOfPages:
+                queued.append(other)
+                continue
+            other.admitted, other.state, other.n_kv = True, SeqState.RUNNING, seq.n_kv
+            other.cached_prefix_tokens = seq.n_kv
+            other.t_admit = self.clock()
+            self.stats.tokens_saved_by_cache += seq.n_kv
+            self.active.insert(at, other)
+            at += 1
+        seq.to_fork = []
+        self.waiting.extendleft(reversed(queued))
 
     # -- planning ----------------------------------------------------------------
     def plan(self) -> list[Planned]:
@@ -267,7 +346,7 @@ class Scheduler:
         end = min(start + budget, seq.prefill_target)
         toks = seq.ctx[start:end]
         # pages for the whole prompt were reserved at admission
-        samples = end >= seq.prefill_target and not seq.output_ids
+        samples = end >= len(seq.ctx)
         return Planned(seq, start, toks, samples)
 
     def _decodes(self) -> list[Planned]:
@@ -275,8 +354,9 @@ class Scheduler:
         planned: list[Planned] = []
         running = [s for s in self.active if s.state == SeqState.RUNNING][: self.max_batch]
         for seq in running:
-            if seq.pending and self._ends_by_count(seq, seq.pending):
-                continue                            # its token in flight is its last
+            if seq.pending and (self._ends_by_count(seq, seq.pending)
+                                or seq.request.grammar is not None):
+                continue                            # its token in flight is its last, or decides
             while seq.state == SeqState.RUNNING:    # else: preempted, or ended while we waited
                 try:
                     mgr.reserve(seq.req_id, seq.n_kv + 1)
@@ -312,24 +392,44 @@ class Scheduler:
         victim.admitted = False
         victim.state = SeqState.WAITING
         victim.preemptions += 1
+        victim.recorded = False
         self.stats.preemptions += 1
         self.waiting.appendleft(victim)
         return victim
+
+    def _masks(self, planned: list[Planned]) -> dict:
+        """What the planned requests' grammars allow next, packed, by request.  A request whose
+        grammar allows nothing any more ends here."""
+        masks = {}
+        for p in planned:
+            grammar = p.seq.request.grammar
+            if grammar is None or not p.samples:
+                continue
+            words = mask_words(grammar.allowed(tuple(p.seq.output_ids)), self.vocab_size)
+            if words is not None and not words.any():
+                p.seq.finish_reason = "grammar"
+                self._finish(p.seq, self.clock())
+                self._late_done.append(p.seq)
+            elif words is not None:
+                masks[p.seq.req_id] = words
+        return masks
 
     # -- running a step -------------------------------------------------------------
     def step(self) -> list[SequenceState]:
         """Plan and launch one step; returns the requests whose end became known in it.  With
         ``pipeline`` the tokens of the step launched here are read in the NEXT call."""
         planned = self.plan()
-        done, self._late_done = self._late_done, []
         # requests that ended while the plan waited for tokens in flight have left it
         planned = [p for p in planned
                    if p.seq.state in (SeqState.PREFILL, SeqState.RUNNING)]
+        masks = self._masks(planned)
+        planned = [p for p in planned if p.seq.state != SeqState.DONE]
+        done, self._late_done = self._late_done, []
         if not planned:
             if self._inflight is not None:
                 done.extend(self._resolve())
                 return done
-            if self.waiting and not self.active:
+            if self.waiting and not self.active and not done:
                 head = self.waiting[0]
                 if head.output_ids:
                     # it outgrew the whole pool while generating: end it with what it has
@@ -345,11 +445,19 @@ class Scheduler:
             return done
         entries = []
         for p in planned:
-            r = p.seq.request
-            entries.append(StepEntry(
-                p.seq.req_id, p.tokens, want=[len(p.tokens) - 1] if p.samples else (),
-                temperature=r.temperature, top_k=r.top_k, seed=r.seed))
+            r, seq = p.seq.request, p.seq
+            entry = StepEntry(
+                seq.req_id, p.tokens, want=[len(p.tokens) - 1] if p.samples else (),
+                temperature=r.temperature, top_k=r.top_k, seed=r.seed)
+            if p.samples:
+                entry.logprobs, entry.rules = r.logprobs, seq.rules
+                entry.allowed = masks.get(seq.req_id)
+                if seq.rules is not None and seq.rules.penalises and not seq.recorded:
+                    entry.history = (r.prompt_ids, list(seq.output_ids))
+            entries.append(entry)
         result = self.step_fn(entries)
+        for p, entry in zip(planned, entries):
+            p.seq.recorded |= entry.history is not None
         n_dec = sum(1 for p in planned if len(p.tokens) == 1 and p.seq.state == SeqState.RUNNING)
         for p in planned:
             seq = p.seq
@@ -362,6 +470,7 @@ class Scheduler:
                     # publish the finished prompt so that others can share it (worker.py:635-645)
                     self.manager.publish(seq.req_id, seq.ctx[: seq.n_kv])
                     seq.state = SeqState.RUNNING
+                    self._fork_samples(seq)
             if p.samples:
                 seq.pending += 1
         self.stats.steps += 1
@@ -387,17 +496,23 @@ class Scheduler:
         planned, result = inflight
         tokens = result.tokens_host() if hasattr(result, "tokens_host") else result
         it = iter(tokens)
+        scores = itertools.repeat(None)
+        if any(p.samples and p.seq.request.logprobs is not None for p in planned) \
+                and hasattr(result, "logprobs_host"):
+            scores = iter(result.logprobs_host())
         done: list[SequenceState] = []
         now = self.clock()
         for p in planned:
             if not p.samples:
                 continue
-            tok = int(next(it))
+            tok, score = int(next(it)), next(scores)
             seq = p.seq
             if seq.state == SeqState.DONE:
                 continue            # ended (or aborted) while this step was in flight
             seq.pending -= 1
             seq.output_ids.append(tok)
+            if score is not None:
+                seq.scores.append(score)
             self.stats.tokens_generated += 1
             if not seq.t_first_token:
                 seq.t_first_token = now
@@ -427,7 +542,17 @@ class Scheduler:
         self.stats.finished += 1
 
     def abort(self, req_id) -> bool:
-        """Drop a request wherever it is; what it holds is given back."""
+        """Drop a request wherever it is; what it holds is given back.  Answers that wait to be
+        forked off it are dropped with it."""
+        for seq in [*self.active, *self.waiting]:
+            for other in seq.to_fork:
+                if req_id in (seq.req_id, other.req_id):
+                    other.state, other.finish_reason = SeqState.DONE, "aborted"
+            forked = [o for o in seq.to_fork if o.state != SeqState.DONE]
+            if seq.req_id != req_id and len(forked) < len(seq.to_fork):
+                seq.to_fork = forked
+                return True
+            seq.to_fork = forked
         for seq in list(self.active):
             if seq.req_id == req_id:
                 self.manager.close(req_id)

@@ -17,11 +17,19 @@ positions, the request of each token, block tables, wanted rows, sampling
 parameters); device to host is one small copy of the sampled tokens and the status
 word, or nothing at all when the caller only wants device logits.  With
 ``cuda_graphs`` the kernels of a step are captured once per size class and replayed.
+
+A step whose entries bring rules (penalties, biases, a grammar's mask) applies them to a copy of
+the wanted logits before it samples, and counts what it sampled into the record the next step's
+penalties go by, all on the device; one whose entries ask for log-probabilities forms them from
+the logits themselves, and they come back behind the tokens in the same copy.  Steps without
+either are what they are without this.
 """
 
 from __future__ import annotations
 
+import contextlib
 import gc
+import itertools
 from dataclasses import dataclass
 from typing import Hashable, Sequence
 
@@ -29,7 +37,8 @@ import numpy as np
 import torch
 
 from ..cache import CacheManager, CacheStorage, GroupSpec, OutOfPages
-from ..kernels.ops import size_class
+from ..kernels.ops import MAX_ALTERNATIVES, TokenHistory, history_words, size_class
+from ..sampling import LogitRules
 
 STATUS_BITS = {1: "a token id outside the vocabulary", 2: "a position outside the table",
                4: "a page number outside the pool", 8: "a kernel pipeline timed out",
@@ -60,6 +69,36 @@ class StepEntry:
     temperature: float = 0.0
     top_k: int = 0
     seed: int = 0
+    rules: LogitRules | None = None
+    # (prompt, generated tokens): the request's record for penalties is begun anew with these
+    # before the step.  Needed once after a request has been opened, if its rules penalise.
+    history: tuple[Sequence[int], Sequence[int]] | None = None
+    allowed: np.ndarray | None = None      # a grammar's mask (packed, see ``sampling.mask_words``)
+    logprobs: int | None = None            # 0: of the sampled token; n: of the n likeliest too
+
+
+@dataclass
+class TokenLogprobs:
+    """Scores of one token: its log-probability, its rank (0: the likeliest), and the likeliest
+    tokens with theirs."""
+
+    logprob: float
+    rank: int
+    top: list[tuple[int, float]]
+
+
+@dataclass(frozen=True)
+class StepExtras:
+    """What a step does beside running tokens and sampling; part of what its shape is."""
+
+    rules: bool = False         # some row has penalties, biases or a mask
+    history: bool = False       # ... penalties: the record is read and added to
+    biases: int = 0             # room for bias entries (a power of two)
+    masks: bool = False         # a mask a wanted row
+    top: int | None = None      # alternatives a row's log-probabilities come with (None: none wanted)
+
+    def score_ints(self, rows: int) -> int:
+        return 0 if self.top is None else rows * (2 + 2 * self.top)
 
 
 @dataclass
@@ -73,6 +112,9 @@ class StepResult:
     _host: torch.Tensor | None = None
     _copied: "torch.cuda.Event | None" = None
     _block: int | None = None            # the metadata block of a step whose copies use side streams
+    _class_rows: int = 0                 # wanted rows with their padding: the status word's place
+    _top: int | None = None              # alternatives per row behind it
+    _asked: list[int | None] | None = None      # ... and how many each row asked for
 
     def start_fetch(self) -> None:
         """Enqueue the device-to-host copy of the sampled tokens (and the status word) behind
@@ -90,11 +132,31 @@ class StepResult:
         self.start_fetch()
         if self._copied is not None:
             self._copied.synchronize()
-        n = self.tokens.shape[0]
-        host = self._host.tolist()          # [bucketed rows..., status word]
-        if host[-1]:
-            self._runner.raise_status(host[-1])
+        n, w = self.tokens.shape[0], self._class_rows
+        host = self._host[:w + 1].tolist()  # [bucketed rows..., status word]
+        if host[w]:
+            self._runner.raise_status(host[w])
         return host[:n]
+
+    def logprobs_host(self) -> list[TokenLogprobs | None]:
+        """Per sampled token its scores, as far as its entry asked for them (they came back with
+        the tokens: call this when those have been read, before four later steps' have)."""
+        if self._top is None:
+            return [None] * len(self.rows)
+        self.start_fetch()
+        if self._copied is not None:
+            self._copied.synchronize()
+        w, top = self._class_rows, self._top
+        at = w + 1
+        host = self._host.numpy()
+        logprob = host[at:at + w].view(np.float32)
+        rank = host[at + w:at + 2 * w]
+        ids = host[at + 2 * w:at + (2 + top) * w].reshape(w, top)
+        lps = host[at + (2 + top) * w:at + (2 + 2 * top) * w].view(np.float32).reshape(w, top)
+        return [None if n is None else
+                TokenLogprobs(float(logprob[i]), int(rank[i]),
+                              list(zip(ids[i, :n].tolist(), lps[i, :n].tolist())))
+                for i, n in enumerate(self._asked)]
 
 
 @dataclass
@@ -113,8 +175,10 @@ class CacheView:
 class Layout:
     """Offsets of the sections of the packed int32 metadata block for one size class."""
 
-    def __init__(self, T: int, R: int, W: int, max_pages: Sequence[int], plan_ints: int):
+    def __init__(self, T: int, R: int, W: int, max_pages: Sequence[int], plan_ints: int,
+                 extras: StepExtras = StepExtras(), vocab: int = 0):
         self.T, self.R, self.W = T, R, W
+        self.extras, self.words = extras, history_words(vocab)
         self.max_pages = tuple(max_pages)
         off = 0
 
@@ -134,6 +198,12 @@ class Layout:
         self.tables = [take(R * mp) for mp in self.max_pages]
         self.plan = take(plan_ints)
         self.plan_ints = plan_ints
+        if extras.rules:
+            self.rule_slot, self.rule_numbers = take(W), [take(W) for _ in range(3)]
+            self.bias_start = take(W + 1)
+            self.bias_ids, self.bias_values = take(extras.biases), take(extras.biases)
+            self.mask_row = take(W)
+            self.masks = take(W * self.words if extras.masks else 0)
         self.total = off
 
 
@@ -164,6 +234,19 @@ class StepContext:
         self.samp_seed_hi = meta[L.samp_seed_hi:L.samp_seed_hi + L.W]
         self.samp_pos = meta[L.samp_pos:L.samp_pos + L.W]
         self.samp_slot = meta[L.samp_slot:L.samp_slot + L.W]
+        self.extras = L.extras
+        if L.extras.rules:
+            part = lambda o, n: meta[o:o + n]                                # noqa: E731
+            self.rule_slot = part(L.rule_slot, L.W)
+            self.repetition, self.presence, self.frequency = (
+                part(o, L.W).view(torch.float32) for o in L.rule_numbers)
+            nb = L.extras.biases
+            self.bias_start = part(L.bias_start, L.W + 1) if nb else None
+            self.bias_ids = part(L.bias_ids, nb) if nb else None
+            self.bias_values = part(L.bias_values, nb).view(torch.float32) if nb else None
+            self.mask_row = part(L.mask_row, L.W) if L.extras.masks else None
+            self.masks = (part(L.masks, L.W * L.words).view(L.W, L.words) if L.extras.masks
+                          else None)
         self.feedback = runner.feedback
         self.tables = [meta[o:o + L.R * mp].view(L.R, mp)
                        for o, mp in zip(L.tables, L.max_pages)]
@@ -288,6 +371,9 @@ class Runner:
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         # the token each request sampled last, by state slot: what FROM_DEVICE reads
         self.feedback = torch.zeros(max(1, max_requests), dtype=torch.int32, device=self.device)
+        # the tokens each state slot's request holds, for penalties; made when first needed
+        self.history: TokenHistory | None = None
+        self._recorded: set[int] = set()      # slots whose record has been begun
         self._fetch_ring: list[torch.Tensor] = []
         self._fetch_next = 0
         if hasattr(ops, "status"):
@@ -329,21 +415,77 @@ class Runner:
         """Every request starts on zeroed state, whoever opened it (this runner, the scheduler
         at admission or after a preemption): the manager calls this for each slot it hands
         out."""
+        self._recorded.discard(slot)
         for st in self.storage.states.values():
             st[slot].zero_()
 
     def close(self, req_id) -> None:
         self.manager.close(req_id)
 
+    def _on_device(self):
+        """The runner's device as the current one."""
+        return torch.cuda.device(self.device) if self.cuda else contextlib.nullcontext()
+
+    def fork(self, req_id, child_id) -> None:
+        """Open ``child_id`` as a copy of ``req_id`` as it stands: full pages are shared, the rows
+        of a partly filled last page, the mixers' state, the token sampled last and the record
+        for penalties are copied on the device, behind what has been launched.  Raises
+        :class:`OutOfPages` with nothing changed."""
+        mgr = self.manager
+        with self._on_device():
+            copies = mgr.fork(req_id, child_id)
+            of, to = mgr.slot(req_id), mgr.slot(child_id)
+            for pool, pairs in zip(self.storage.pools, copies):
+                if pairs:
+                    self.ops.copy_pages(pool, pool, [d for _s, d, _n in pairs],
+                                        [s for s, _d, _n in pairs], [n for _s, _d, n in pairs])
+            rows = list(self.storage.states.values()) + [self.feedback.view(-1, 1).view(torch.float32)]
+            if of in self._recorded:
+                rows += [t.view(torch.float32) for t in self.history.tensors()]
+                self._recorded.add(to)
+            for t in rows:                     # a row a slot: a page of one row
+                view = t.view(1, t.shape[0], 1, 1, 1, -1)
+                self.ops.copy_pages(view, view, [to], [of])
+
+    def resize_cache(self, num_pages: int) -> None:
+        """Give the page groups pools of the size ``num_pages`` stands for when a runner is made.
+        Live requests keep their pages (moved to the lowest numbers of the new pools), published
+        prefixes as far as they fit.  Raises :class:`OutOfPages` with nothing changed when the
+        live requests' pages do not fit; both pools of a group exist while its pages move.  The
+        longest request the runner takes (``max_positions``) stays what it was."""
+        mgr, model = self.manager, self.model
+        sizes = [-(-num_pages // g.stride) + mgr.max_requests if g.stride > 1 else num_pages
+                 for g in mgr.groups]
+        for pool, n in zip(mgr.pools, sizes):
+            if n <= 0 or pool.num_held() > n:
+                raise OutOfPages(f"{pool.num_held()} pages are held: they do not fit {n}")
+        with self._on_device():
+            if self.cuda:
+                torch.cuda.synchronize(self.device)
+            new = [torch.zeros((old.shape[0], n, *old.shape[2:]), dtype=old.dtype, device=old.device)
+                   for old, n in zip(self.storage.pools, sizes)]
+            self._graphs.clear()               # they point into the old pools
+            moves = mgr.resize(sizes)
+            for gi, moved in enumerate(moves):
+                if moved:
+                    self.ops.copy_pages(new[gi], self.storage.pools[gi], list(moved.values()),
+                                        list(moved))
+                self.storage.pools[gi] = new[gi]
+            if self.fused is not None:
+                from ..parts.fused import plan_fused_decode
+                self.fused = plan_fused_decode(model, self.ops, self.storage, mgr.page_size)
+            if self.cuda:
+                torch.cuda.synchronize(self.device)     # the old pools are free from here on
+
     # -- the step -----------------------------------------------------------------
-    def _layout(self, T, R, W) -> Layout:
-        key = (T, R, W)
+    def _layout(self, T, R, W, extras: StepExtras = StepExtras()) -> Layout:
+        key = (T, R, W, extras)
         lay = self._layouts.get(key)
         if lay is None:
             plan_ints = 0
             if hasattr(self.ops, "attention_plan_ints"):
                 plan_ints = self.ops.attention_plan_ints(T, R)
-            lay = Layout(T, R, W, self.max_pages, plan_ints)
+            lay = Layout(T, R, W, self.max_pages, plan_ints, extras, self.model.spec.vocab_size)
             self._layouts[key] = lay
         return lay
 
@@ -399,6 +541,7 @@ class Runner:
             starts.append(start)
             n_tok += n
             n_want += len(e.want)
+        extras = self._extras(entries) if sample else StepExtras()
         # Nothing above changed anything.  Requests the cache does not know are opened here and
         # pages are reserved entry by entry; if one cannot be had, what this step took so far
         # is given back, so that a refused step leaves the cache as it found it.
@@ -424,11 +567,11 @@ class Runner:
             W = size_class(n_want) if n_want else 0
         else:
             T, R, W = n_tok, len(entries), n_want
-        lay = self._layout(T, R, W)
+        lay = self._layout(T, R, W, extras)
         # The second block (and the second graph of a shape) is for shapes that keep coming
         # back, such as a decode batch of a fixed size: capturing a graph costs what a
         # thousand overlapped uploads save, so a shape earns it with use.
-        shape = (T, R, W, bool(sample))
+        shape = (T, R, W, bool(sample), extras)
         uses = self._shape_uses.get(shape, 0) + 1
         self._shape_uses[shape] = uses
         hot = self._copy_stream is not None and uses > self.hot_shape_uses
@@ -489,6 +632,8 @@ class Runner:
                 w_i += 1
             host_batch.append((e.req_id, slot, start, n))
             t += n
+        if extras.rules:
+            self._pack_rules(hm, lay, entries)
         plan_shape = None
         if lay.plan_ints:
             plan_shape = self.ops.plan_attention(hm[lay.plan:lay.plan + lay.plan_ints],
@@ -501,13 +646,17 @@ class Runner:
             sides = self.ops.plan_sides(host_batch, self.model.portion_limits)
 
         # ---- device side -------------------------------------------------------------
-        greedy = all(e.temperature <= 0.0 for e in entries)
-        key = (T, R, W, bool(sample), plan_shape, sides, greedy, parity)
-        dev = self._dev_meta.get((T, R, W, parity))
+        # (tokens the head or a fused step picks know no rules, and bring no scores)
+        greedy = (all(e.temperature <= 0.0 for e in entries) and not extras.rules
+                  and extras.top is None)
+        key = (T, R, W, bool(sample), extras, plan_shape, sides, greedy, parity)
+        if extras.history:
+            self._begin_histories(entries)
+        dev = self._dev_meta.get((T, R, W, extras, parity))
         fresh = dev is None
         if fresh:
             dev = torch.zeros(lay.total, dtype=torch.int32, device=self.device)
-            self._dev_meta[(T, R, W, parity)] = dev
+            self._dev_meta[(T, R, W, extras, parity)] = dev
         if not hot:
             # This copy is also what separates steps on the stream: it is not a kernel, so no
             # kernel of this step, however early programmatic dependent launch lets it start,
@@ -570,8 +719,12 @@ class Runner:
                 if ran_eagerly:
                     kept = self.feedback.clone()
                     kept_state = {k: st.clone() for k, st in self.storage.states.items()}
+                    counted = self.history.tensors()[1:] if extras.history else ()
+                    kept_counts = [t.clone() for t in counted]
                     self._forward(ctx, sample)
                     self.feedback.copy_(kept)
+                    for t, old in zip(counted, kept_counts):
+                        t.copy_(old)
                     for k, st in kept_state.items():
                         self.storage.states[k].copy_(st)
                 torch.cuda.synchronize(self.device)
@@ -612,7 +765,115 @@ class Runner:
             tokens=None if tokens is None else tokens[:n_want],
             rows=rows, n_tokens=n_tok,
             _with_status=None if tokens is None else tokens, _runner=self,
-            _block=parity if hot else None)
+            _block=parity if hot else None, _class_rows=W,
+            _top=None if tokens is None else extras.top,
+            _asked=[e.logprobs for e in entries for _ in e.want])
+
+    def _extras(self, entries) -> StepExtras:
+        """What the entries ask for beside tokens; refuses what cannot be given, before anything
+        changes."""
+        vocab = self.model.spec.vocab_size
+        rules = history = masks = False
+        biases, top = 0, None
+        for e in entries:
+            if not e.want:
+                continue
+            r = e.rules
+            if r is not None or e.allowed is not None:
+                if len(e.want) > 1 or e.want[0] != len(e.tokens) - 1:
+                    raise StepError(f"request {e.req_id!r}: rules act on its next token alone, "
+                                    f"places {list(e.want)} are wanted")
+            if r is not None and not r.neutral:
+                try:
+                    r.check(vocab)
+                except ValueError as exc:
+                    raise StepError(f"request {e.req_id!r}: {exc}") from None
+                rules = True
+                biases += len(r.bias)
+                if r.penalises:
+                    history = True
+                    if e.history is None and (e.req_id not in self.manager
+                                              or self.manager.slot(e.req_id) not in self._recorded):
+                        raise StepError(f"request {e.req_id!r}: penalties need its history")
+                    for t in itertools.chain.from_iterable(e.history or ()):
+                        if not 0 <= t < vocab:
+                            raise StepError(f"request {e.req_id!r}: token id outside [0, {vocab}) "
+                                            "in its history")
+            if e.allowed is not None:
+                a = e.allowed
+                if not isinstance(a, np.ndarray) or a.dtype != np.int32 \
+                        or a.shape != (history_words(vocab),):
+                    raise StepError(f"request {e.req_id!r}: its mask is not "
+                                    f"{history_words(vocab)} int32 words")
+                rules = masks = True
+            if e.logprobs is not None:
+                if not 0 <= e.logprobs <= min(MAX_ALTERNATIVES, vocab):
+                    raise StepError(f"request {e.req_id!r}: {e.logprobs} alternatives; at most "
+                                    f"{min(MAX_ALTERNATIVES, vocab)}")
+                top = max(top or 0, e.logprobs)
+        if top:                                # three classes, so that few graphs are captured
+            top = min(8 if top <= 8 else MAX_ALTERNATIVES, vocab)
+        if biases and self.use_graphs:
+            biases = _bucket(biases, 64)
+        return StepExtras(rules, history, biases, masks, top)
+
+    def _pack_rules(self, hm, lay: Layout, entries) -> None:
+        """The rules of the wanted rows, into the metadata block; rows of padding have none."""
+        W, nb = lay.W, lay.extras.biases
+        hm[lay.rule_slot:lay.rule_slot + W] = -1
+        numbers = [hm[o:o + W].view(np.float32) for o in lay.rule_numbers]
+        for a, neutral in zip(numbers, (1.0, 0.0, 0.0)):
+            a[:] = neutral
+        start = hm[lay.bias_start:lay.bias_start + W + 1]
+        start[:] = 0
+        ids = hm[lay.bias_ids:lay.bias_ids + nb]
+        values = hm[lay.bias_values:lay.bias_values + nb].view(np.float32)
+        mask_row = hm[lay.mask_row:lay.mask_row + W]
+        mask_row[:] = -1
+        w = at = 0
+        for e in entries:
+            for _ in e.want:
+                r = e.rules
+                if r is not None and r.penalises:
+                    hm[lay.rule_slot + w] = self.manager.slot(e.req_id)
+                    numbers[0][w], numbers[1][w], numbers[2][w] = (r.repetition, r.presence,
+                                                                   r.frequency)
+                if r is not None and r.bias:
+                    n = len(r.bias)
+                    ids[at:at + n] = list(r.bias.keys())
+                    values[at:at + n] = list(r.bias.values())
+                    at += n
+                if e.allowed is not None:
+                    mask_row[w] = w
+                    o = lay.masks + w * lay.words
+                    hm[o:o + lay.words] = e.allowed
+                w += 1
+                start[w] = at
+        start[w:] = at
+
+    def _begin_histories(self, entries) -> None:
+        """Begin the records that entries bring tokens for, in one launch."""
+        if self.history is None:
+            self.history = TokenHistory.zeros(max(1, self.manager.max_requests),
+                                              self.model.spec.vocab_size, self.device)
+        begun = [e for e in entries if e.want and e.history is not None and e.rules is not None
+                 and e.rules.penalises]
+        if not begun:
+            return
+        slots = [self.manager.slot(e.req_id) for e in begun]
+        tokens, start, n_prompt = [], [0], []
+        for e in begun:
+            tokens += [*e.history[0], *e.history[1]]
+            start.append(len(tokens))
+            n_prompt.append(len(e.history[0]))
+        block = torch.tensor(slots + start + n_prompt + tokens, dtype=torch.int32)
+        if self.cuda:
+            block = block.pin_memory().to(self.device, non_blocking=True)
+        k = len(begun)
+        self.ops.history_begin(self.history, block[:k], block[3 * k + 1:], block[k:2 * k + 1],
+                               block[2 * k + 1:3 * k + 1])
+        self.kernel_launches += 1
+        self._recorded.update(slots)
 
     def _forward(self, ctx: StepContext, sample: bool):
         ctx.fused_tokens = None
@@ -622,7 +883,8 @@ class Runner:
         if sample and logits is not None:
             # one extra element carries the status word, so that one copy brings both back
             W = ctx.n_logit_rows
-            tokens = ctx.buffer(ctx.tokens_name, (W + 1,), torch.int32)
+            extras = ctx.extras
+            tokens = ctx.buffer(ctx.tokens_name, (W + 1 + extras.score_ints(W),), torch.int32)
             if ctx.fused_tokens is not None and ctx.greedy_only:
                 # the step ran as one kernel, which also chose the tokens (argmax, lowest
                 # index on ties), kept them for the requests and stored the status word
@@ -630,12 +892,38 @@ class Runner:
             more = {}
             if getattr(self.ops, "takes_status_word", False):
                 more["status_word"] = self.status          # stored to tokens[W] by the kernel
-            self.ops.sample(tokens, logits, ctx.samp_temp, ctx.samp_topk, ctx.samp_seed_lo,
+            ruled = self._apply_rules(ctx, logits) if extras.rules else logits
+            self.ops.sample(tokens, ruled, ctx.samp_temp, ctx.samp_topk, ctx.samp_seed_lo,
                             ctx.samp_seed_hi, ctx.samp_pos, feedback=self.feedback,
                             feedback_slot=ctx.samp_slot, **more)
+            if extras.history:
+                self.ops.history_add(self.history, ctx.rule_slot, tokens[:W])
+            if extras.top is not None:
+                self._score(tokens, logits, W, extras.top)
             if not more:
-                tokens[W:].copy_(self.status)
+                tokens[W:W + 1].copy_(self.status)
         return logits, tokens
+
+    def _apply_rules(self, ctx: StepContext, logits: torch.Tensor) -> torch.Tensor:
+        """The logits under the rows' rules; the step's own logits stay as they are."""
+        out = ctx.buffer("ruled_logits", tuple(logits.shape), torch.float32)
+        record = (self.history, ctx.rule_slot, ctx.repetition, ctx.presence, ctx.frequency) \
+            if ctx.extras.history else ()
+        self.ops.logit_rules(out, logits, *record, bias_start=ctx.bias_start,
+                             bias_ids=ctx.bias_ids, bias_values=ctx.bias_values, mask=ctx.masks,
+                             mask_row=ctx.mask_row)
+        return out
+
+    def _score(self, tokens: torch.Tensor, logits: torch.Tensor, W: int, top: int) -> None:
+        """Log-probabilities of the sampled tokens, into the words behind the status word."""
+        at = W + 1
+        flat = tokens.view(torch.float32)
+        alternatives = ()
+        if top:
+            alternatives = (tokens[at + 2 * W:at + (2 + top) * W].view(W, top),
+                            flat[at + (2 + top) * W:at + (2 + 2 * top) * W].view(W, top))
+        self.ops.token_logprobs(flat[at:at + W], tokens[at + W:at + 2 * W], logits, tokens[:W],
+                                *alternatives)
 
     def _fetch(self, dev: torch.Tensor, block: int | None = None):
         """Start copying ``dev`` (int32) to pinned host memory behind the work enqueued so far;

@@ -1,0 +1,105 @@
+"""What a request may say: penalties for tokens it repeats, biases of single tokens, and
+grammars that rule tokens out.
+
+The arithmetic is :meth:`CudaOps.logit_rules`'s, in this order: a token seen in the prompt or
+answer has its logit divided by ``repetition`` (multiplied where it is not positive); one
+generated c > 0 times loses ``frequency * c + presence``; a biased token gains its bias; a token
+that the grammar rules out becomes -inf.
+
+A *grammar* is any object with ``allowed(output_ids)``: asked before every token with the tokens
+generated so far, it says which may come next — ``None`` (any), a packed mask
+(``ceil(vocab / 32)`` 32-bit words, bit v % 32 of word v // 32), truth values over the
+vocabulary, or token ids.  An answer that allows nothing ends the request.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass, field
+from typing import Mapping, Sequence
+
+import numpy as np
+
+
+@dataclass(frozen=True)
+class LogitRules:
+    repetition: float = 1.0
+    presence: float = 0.0
+    frequency: float = 0.0
+    bias: Mapping[int, float] = field(default_factory=dict)
+
+    @property
+    def penalises(self) -> bool:
+        """Whether the record of the request's tokens is needed."""
+        return self.repetition != 1.0 or self.presence != 0.0 or self.frequency != 0.0
+
+    @property
+    def neutral(self) -> bool:
+        return not self.penalises and not self.bias
+
+    def check(self, vocab: int | None = None) -> None:
+        """Raise ValueError for numbers no request can mean."""
+        if not (math.isfinite(self.repetition) and self.repetition > 0):
+            raise ValueError(f"repetition penalty {self.repetition} is not a positive number")
+        for name in ("presence", "frequency"):
+            if not math.isfinite(getattr(self, name)):
+                raise ValueError(f"{name} penalty {getattr(self, name)} is not a finite number")
+        for token, value in self.bias.items():
+            if isinstance(token, bool) or not isinstance(token, (int, np.integer)) or token < 0 \
+                    or (vocab is not None and token >= vocab):
+                raise ValueError(f"bias of token {token!r}, which the vocabulary does not have")
+            if math.isnan(value) or value == math.inf:
+                raise ValueError(f"bias {value} of token {token}: neither a number nor -inf")
+
+
+def mask_words(allowed, vocab: int) -> np.ndarray | None:
+    """What a grammar's ``allowed`` answered as packed int32 words (None: any token)."""
+    if allowed is None:
+        return None
+    words = -(-vocab // 32)
+    if isinstance(allowed, np.ndarray) and allowed.dtype != bool and allowed.ndim == 1 \
+            and allowed.dtype.itemsize == 4 and allowed.dtype.kind in "iu":
+        if allowed.shape[0] != words:
+            raise ValueError(f"a mask of {allowed.shape[0]} words for {vocab} tokens ({words} words)")
+        out = allowed.astype(np.uint32, copy=True)
+        if vocab % 32:
+            out[-1] &= np.uint32((1 << (vocab % 32)) - 1)
+        return out.view(np.int32)
+    flags = np.zeros(words * 32, dtype=bool)
+    if isinstance(allowed, np.ndarray) and allowed.dtype == bool:
+        if allowed.shape != (vocab,):
+            raise ValueError(f"truth values of shape {allowed.shape} for {vocab} tokens")
+        flags[:vocab] = allowed
+    else:
+        ids = np.fromiter((int(t) for t in allowed), dtype=np.int64)
+        if ids.size and (ids.min() < 0 or ids.max() >= vocab):
+            raise ValueError(f"a grammar allows a token outside [0, {vocab})")
+        flags[ids] = True
+    return np.packbits(flags, bitorder="little").view(np.int32)
+
+
+class OneOf:
+    """The grammar of a choice: the answer is one of the given token sequences, and then
+    ``end`` (the end-of-sequence token, say) if one is given."""
+
+    def __init__(self, sequences: Sequence[Sequence[int]], end: int | None = None):
+        if not sequences or any(len(s) == 0 for s in sequences):
+            raise ValueError("a choice needs sequences, none of them empty")
+        self._root: dict = {}
+        self._end = end
+        for s in sequences:
+            node = self._root
+            for t in s:
+                node = node.setdefault(int(t), {})
+            node[None] = True                      # a sequence ends here
+
+    def allowed(self, output_ids: Sequence[int]) -> list[int]:
+        node = self._root
+        for t in output_ids:
+            if t not in node:
+                return []
+            node = node[t]
+        ids = [t for t in node if t is not None]
+        if None in node and self._end is not None:
+            ids.append(self._end)
+        return ids
