@@ -9,6 +9,7 @@
 // The record of a slot is two bit rows over the vocabulary (bit v % 32 of word v / 32: v stands in
 // the prompt; v has been generated) and a row of counts, read only where the second bit is set.
 #include "common.cuh"
+#include <string.h>
 
 namespace hs {
 
@@ -298,32 +299,53 @@ __global__ void history_add_kernel(int* output, int* counts, int vocab, int word
 
 }  // namespace hs
 
-// prompt / output / counts / slots (and the three penalties) are null together, so are the bias's
-// three and the mask's two.  bias_start holds rows + 1 offsets into n_bias entries; of an id that a
-// row lists twice the last entry counts.  out may be logits itself.
-HS_EXPORT int hs_logit_rules(float* out, const float* logits, int rows, int vocab, const int* prompt,
-                             const int* output, const int* counts, int n_slots, const int* slots,
-                             const float* repetition, const float* presence, const float* frequency,
-                             const int* bias_start, const int* bias_ids, const float* bias_values,
-                             int n_bias, const int* mask, int n_masks, const int* mask_row,
-                             int* status, void* stream) {
-  if (!out || !logits || !status || vocab <= 0) return HS_ERR_ARGUMENT;
-  if (slots && (!prompt || !output || !counts || !repetition || !presence || !frequency))
+// The arguments of hs_logit_rules, eight bytes each.  The record's three tensors, slots and the
+// three penalties are null together, so are the bias's three and the mask's two.  bias_start holds
+// rows + 1 offsets into n_bias entries; of an id that a row lists twice the last entry counts.  out
+// may be logits itself.
+struct HsLogitRules {
+  float* out;
+  const float* logits;
+  long long rows, vocab;
+  const int *prompt, *output, *counts;
+  long long n_slots;
+  const int* slots;
+  const float *repetition, *presence, *frequency;
+  const int *bias_start, *bias_ids;
+  const float* bias_values;
+  long long n_bias;
+  const int* mask;
+  long long n_masks;
+  const int* mask_row;
+  int* status;
+};
+static_assert(sizeof(HsLogitRules) == 20 * 8, "");
+
+HS_EXPORT int hs_logit_rules(const HsLogitRules* in, void* stream) {
+  if (!in) return HS_ERR_ARGUMENT;
+  HsLogitRules a;
+  memcpy(&a, in, sizeof a);
+  if (!a.out || !a.logits || !a.status || a.vocab <= 0) return HS_ERR_ARGUMENT;
+  if (a.slots && (!a.prompt || !a.output || !a.counts || !a.repetition || !a.presence || !a.frequency))
     return HS_ERR_ARGUMENT;
-  if (bias_start && (!bias_ids || !bias_values)) return HS_ERR_ARGUMENT;
-  if ((mask == nullptr) != (mask_row == nullptr)) return HS_ERR_ARGUMENT;
-  if (rows <= 0) return HS_OK;
-  if (rows > 65535) return HS_ERR_UNSUPPORTED;
+  if (a.bias_start && (!a.bias_ids || !a.bias_values)) return HS_ERR_ARGUMENT;
+  if ((a.mask == nullptr) != (a.mask_row == nullptr)) return HS_ERR_ARGUMENT;
+  if (a.rows <= 0) return HS_OK;
+  if (a.rows > 65535 || a.vocab > 0x7fff0000 || a.n_slots > 0x7fffffff || a.n_bias > 0x7fffffff ||
+      a.n_masks > 0x7fffffff)
+    return HS_ERR_UNSUPPORTED;
+  const int rows = (int)a.rows, vocab = (int)a.vocab;
   // as many tiles as run at a time, none narrower than a round of a block's loads
   const int fit = hs::LR_BLOCKS * hs_sm_count(), tiles = fit / rows > 1 ? fit / rows : 1;
   int tile = ((vocab + tiles - 1) / tiles + 1023) / 1024 * 1024;
   if (tile > hs::LR_MOST) tile = hs::LR_MOST;
-  const hs::LogitRules args{out, logits, vocab, (vocab + 31) / 32, tile, prompt, output, counts, n_slots,
-                            slots, repetition, presence, frequency, bias_start, bias_ids, bias_values,
-                            n_bias, mask, n_masks, mask_row, status};
+  const hs::LogitRules args{a.out, a.logits, vocab, (vocab + 31) / 32, tile, a.prompt, a.output, a.counts,
+                            (int)a.n_slots, a.slots, a.repetition, a.presence, a.frequency, a.bias_start,
+                            a.bias_ids, a.bias_values, (int)a.n_bias, a.mask, (int)a.n_masks, a.mask_row,
+                            a.status};
   const dim3 grid((vocab + tile - 1) / tile, rows);
   const cudaError_t e =
-      bias_start ? hs_launch(hs::logit_rules_kernel<true>, grid, dim3(hs::LR_THREADS), 0,
+      a.bias_start ? hs_launch(hs::logit_rules_kernel<true>, grid, dim3(hs::LR_THREADS), 0,
                              (cudaStream_t)stream, hs_pdl_enabled(), args)
                  : hs_launch(hs::logit_rules_kernel<false>, grid, dim3(hs::LR_THREADS), 0,
                              (cudaStream_t)stream, hs_pdl_enabled(), args);

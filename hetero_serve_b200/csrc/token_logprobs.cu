@@ -22,6 +22,7 @@ constexpr int TL_TOP = 32;                // a warp's lanes hold the alternative
 constexpr int TL_GROUPS = 32;             // of threads, whose maxima give the bound
 constexpr int TL_INFLIGHT = 4;            // 16-byte loads a thread has under way
 constexpr int TL_CAND = 1024;             // logits looked at again at a time
+constexpr int TL_FEW = 256;               // ... that are put in order by counting
 
 typedef unsigned long long tl_key_t;
 
@@ -285,14 +286,14 @@ token_logprobs_kernel(float* __restrict__ logprob, int* __restrict__ rank, int* 
     if (holds && own_order >= reach) s_owner[atomicAdd(&s_owners, 1)] = (uint16_t)tid;
     __syncthreads();
     const int owners = s_owners;
-    bool done = owners * 4 <= TL_CAND;    // else more is equal than a list takes, or nearly so
+    bool done = owners <= TL_FEW;         // else more is equal than a list takes, or nearly so
     if (done) {
       for (int q = tid; q < owners * rounds; q += THREADS)
         again(s_owner[q / rounds], q % rounds, (tl_key_t)reach << 32);
       again_edge((tl_key_t)reach << 32);
       __syncthreads();
       const int found = s_found;
-      done = found <= TL_CAND && found >= min(top, elements);
+      done = found <= TL_FEW && found >= min(top, elements);
       if (done) {
         for (int i = tid; i < found; i += THREADS) {
           const tl_key_t k = s_cand[i];

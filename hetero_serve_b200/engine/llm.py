@@ -24,6 +24,7 @@ from typing import Sequence
 import torch
 
 from ..config import EngineConfig, preset
+from ..kernels.ops import MAX_ALTERNATIVES
 from ..weights import write_model_dir
 from .loading import TORCH_DTYPES, load_model
 from .metrics import RequestRecord, summarise
@@ -123,6 +124,9 @@ class LLMEngine:
         requests, in portions of the engine's token budget, and needs a state slot and pages for
         the text meanwhile (:class:`OutOfPages` otherwise)."""
         runner, text = self.runner, [int(t) for t in token_ids]
+        most = min(MAX_ALTERNATIVES, self.model.spec.vocab_size)
+        if not 0 <= alternatives <= most:
+            raise ValueError(f"{alternatives} alternatives: between 0 and {most}")
         name, out = ("score", next(_scored)), []
         with runner._on_device():
             runner.open(name)

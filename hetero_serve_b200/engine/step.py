@@ -29,7 +29,6 @@ from __future__ import annotations
 
 import contextlib
 import gc
-import itertools
 from dataclasses import dataclass
 from typing import Hashable, Sequence
 
@@ -789,14 +788,15 @@ class Runner:
                 except ValueError as exc:
                     raise StepError(f"request {e.req_id!r}: {exc}") from None
                 rules = True
-                biases += len(r.bias)
+                biases += len(r.bias_ids)
                 if r.penalises:
                     history = True
                     if e.history is None and (e.req_id not in self.manager
                                               or self.manager.slot(e.req_id) not in self._recorded):
                         raise StepError(f"request {e.req_id!r}: penalties need its history")
-                    for t in itertools.chain.from_iterable(e.history or ()):
-                        if not 0 <= t < vocab:
+                    for part in e.history or ():
+                        known = np.asarray(part, dtype=np.int64)
+                        if known.size and not (0 <= int(known.min()) and int(known.max()) < vocab):
                             raise StepError(f"request {e.req_id!r}: token id outside [0, {vocab}) "
                                             "in its history")
             if e.allowed is not None:
@@ -838,10 +838,9 @@ class Runner:
                     hm[lay.rule_slot + w] = self.manager.slot(e.req_id)
                     numbers[0][w], numbers[1][w], numbers[2][w] = (r.repetition, r.presence,
                                                                    r.frequency)
-                if r is not None and r.bias:
-                    n = len(r.bias)
-                    ids[at:at + n] = list(r.bias.keys())
-                    values[at:at + n] = list(r.bias.values())
+                if r is not None and len(r.bias_ids):
+                    n = len(r.bias_ids)
+                    ids[at:at + n], values[at:at + n] = r.bias_ids, r.bias_values
                     at += n
                 if e.allowed is not None:
                     mask_row[w] = w
@@ -863,10 +862,11 @@ class Runner:
         slots = [self.manager.slot(e.req_id) for e in begun]
         tokens, start, n_prompt = [], [0], []
         for e in begun:
-            tokens += [*e.history[0], *e.history[1]]
-            start.append(len(tokens))
+            tokens += e.history
+            start.append(start[-1] + len(e.history[0]) + len(e.history[1]))
             n_prompt.append(len(e.history[0]))
-        block = torch.tensor(slots + start + n_prompt + tokens, dtype=torch.int32)
+        block = torch.from_numpy(np.concatenate(
+            [np.asarray(x, dtype=np.int32) for x in (slots, start, n_prompt, *tokens)]))
         if self.cuda:
             block = block.pin_memory().to(self.device, non_blocking=True)
         k = len(begun)

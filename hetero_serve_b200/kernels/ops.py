@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from array import array
 from ctypes import c_float, c_int, c_void_p
 from dataclasses import dataclass
@@ -267,6 +268,8 @@ def _shares_memory(a, b) -> bool:
     return False
 
 
+_RULES = struct.Struct("20q")      # the arguments of hs_logit_rules, in the order of its struct
+
 _ERRORS = {-1: "unsupported size, type or option", -2: "bad argument"}
 
 _lib = None
@@ -389,7 +392,7 @@ def _declare(lib) -> None:
                                         I, I, F, I, P, P],
         "hs_moe_sorted_scratch": [I, I, I, I, I, I, P, P],
         "hs_sample": [P, P, P, P, P, P, P, I, I, P, P, P, P],
-        "hs_logit_rules": [P, P, I, I, P, P, P, I, P, P, P, P, P, P, P, I, P, I, P, P, P],
+        "hs_logit_rules": [ctypes.c_char_p, P],
         "hs_history_begin": [P, P, P, I, I, P, I, P, I, P, P, P, P],
         "hs_history_add": [P, P, I, I, P, P, I, P, P],
         "hs_token_logprobs": [P, P, P, P, I, P, P, I, I, P, P],
@@ -2780,16 +2783,32 @@ class CudaOps:
                                   self._stream()), "sample")
 
     # -- rules on logits, and the record of tokens they go by ------------------------------------
-    def _fits(self, what, t, name, dtype, rows):
-        """Refuse anything but a vector of ``rows`` numbers or more on this object's device."""
-        if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == 1
-                and t.get_device() == self.device.index and t.is_contiguous()
-                and t.numel() >= rows):
-            return
+    def _at(self, what, t, name, dtype, rows):
+        """Where a vector of ``rows`` numbers or more lies on this object's device; anything else
+        is refused."""
+        try:
+            if (t.dtype is dtype and t.numel() >= rows and t.dim() == 1
+                    and t.get_device() == self.device.index and t.is_contiguous()):
+                return t.data_ptr()
+        except AttributeError:
+            pass
         _want(t, name, dtype, 1)
         if t.numel() < rows:
             raise KernelError(f"{what}: {name} shorter than the rows")
         self._drives(what, t)
+        return t.data_ptr()
+
+    def _matrix(self, what, t, name, dtype):
+        """Where a matrix lies on this object's device, and its sizes."""
+        try:
+            if (t.dtype is dtype and t.dim() == 2 and t.get_device() == self.device.index
+                    and t.is_contiguous()):
+                return t.data_ptr(), *t.shape
+        except AttributeError:
+            pass
+        _want(t, name, dtype, 2)
+        self._drives(what, t)
+        return t.data_ptr(), *t.shape
 
     def _drives(self, what, *tensors):
         """Kernels run on this object's device, which has to be the current one."""
@@ -2802,11 +2821,14 @@ class CudaOps:
                               f"kernels drive {self.device}")
 
     def _history(self, what, history):
+        """Where the three tensors of a record lie, its slots and its vocabulary."""
         if not isinstance(history, TokenHistory):
             raise KernelError(f"{what}: history must be a TokenHistory, "
                               f"got {type(history).__name__}")
-        self._drives(what, history.counts)
-        return history.counts.shape
+        counts = history.counts
+        self._drives(what, counts)
+        return (history.prompt.data_ptr(), history.output.data_ptr(), counts.data_ptr(),
+                *counts.shape)
 
     def history_begin(self, history, slots, tokens, start, n_prompt):
         """For every k: slot ``slots[k]`` gets the record of ``tokens[start[k]:start[k + 1]]``,
@@ -2814,31 +2836,29 @@ class CudaOps:
         slot held before is gone; other slots stay.  A slot below zero is skipped; of two rows
         of one slot the last counts.  Token ids outside the vocabulary are left out and
         reported in the status word."""
-        what = "history_begin"
-        n_slots, vocab = self._history(what, history)
-        self._fits(what, slots, "slots", torch.int32, 0)
+        what, i32 = "history_begin", torch.int32
+        record = self._history(what, history)
+        at = self._at(what, slots, "slots", i32, 0)
         rows = slots.shape[0]
-        self._fits(what, tokens, "tokens", torch.int32, 0)
-        self._fits(what, n_prompt, "n_prompt", torch.int32, rows)
-        self._fits(what, start, "start", torch.int32, rows + 1)
+        tokens_at = self._at(what, tokens, "tokens", i32, 0)
+        prompt_at = self._at(what, n_prompt, "n_prompt", i32, rows)
+        start_at = self._at(what, start, "start", i32, rows + 1)
         self.launches += 1
         _check(self.lib.hs_history_begin(
-            _ptr(history.prompt), _ptr(history.output), _ptr(history.counts), n_slots, vocab,
-            _ptr(slots), rows, _ptr(tokens), tokens.shape[0], _ptr(start), _ptr(n_prompt),
-            _ptr(self._status_of(slots)), self._stream()), "history_begin")
+            *record, at, rows, tokens_at, tokens.shape[0], start_at, prompt_at,
+            self._status_of(slots).data_ptr(), self._stream()), what)
 
     def history_add(self, history, slots, tokens):
         """Count ``tokens[i]`` as generated in slot ``slots[i]`` (below zero: skipped), for as
         many rows as ``slots`` has."""
         what = "history_add"
-        n_slots, vocab = self._history(what, history)
-        self._fits(what, slots, "slots", torch.int32, 0)
+        _prompt, output, counts, n_slots, vocab = self._history(what, history)
+        at = self._at(what, slots, "slots", torch.int32, 0)
         rows = slots.shape[0]
-        self._fits(what, tokens, "tokens", torch.int32, rows)
+        tokens_at = self._at(what, tokens, "tokens", torch.int32, rows)
         self.launches += 1
-        _check(self.lib.hs_history_add(
-            _ptr(history.output), _ptr(history.counts), n_slots, vocab, _ptr(slots), _ptr(tokens),
-            rows, _ptr(self._status_of(slots)), self._stream()), "history_add")
+        _check(self.lib.hs_history_add(output, counts, n_slots, vocab, at, tokens_at, rows,
+                                       self._status_of(slots).data_ptr(), self._stream()), what)
 
     def logit_rules(self, out, logits, history=None, slots=None, repetition=None, presence=None,
                     frequency=None, *, bias_start=None, bias_ids=None, bias_values=None, mask=None,
@@ -2856,59 +2876,51 @@ class CudaOps:
 
         The arithmetic on a token is done in 64 bits and rounded once.  Ids, records and masks
         outside their tables are left out and reported in the status word."""
-        what = "logit_rules"
-        _want(logits, "logits", torch.float32, 2)
-        _want(out, "out", torch.float32, 2)
-        self._drives(what, logits, out)
-        rows, vocab = logits.shape
-        if out.shape != logits.shape:
-            raise KernelError(f"logit_rules: out {tuple(out.shape)} for logits {(rows, vocab)}")
-        a, b = out.data_ptr(), logits.data_ptr()
+        what, i32, f32 = "logit_rules", torch.int32, torch.float32
+        b, rows, vocab = self._matrix(what, logits, "logits", f32)
+        a, *sizes = self._matrix(what, out, "out", f32)
+        self._drives(what)
+        if sizes != [rows, vocab]:
+            raise KernelError(f"logit_rules: out {tuple(sizes)} for logits {(rows, vocab)}")
         if a != b and abs(a - b) < 4 * rows * vocab:
             raise KernelError("logit_rules: out overlaps the logits without being them")
-        n_slots = n_masks = n_bias = 0
-        bits = (None, None, None)
+        penalties = (0,) * 8
         if history is not None:
-            n_slots, known = self._history(what, history)
+            *bits, n_slots, known = self._history(what, history)
             if known != vocab:
                 raise KernelError(f"logit_rules: a history of {known} tokens for {vocab} logits")
-            self._fits(what, slots, "slots", torch.int32, rows)
-            self._fits(what, repetition, "repetition", torch.float32, rows)
-            self._fits(what, presence, "presence", torch.float32, rows)
-            self._fits(what, frequency, "frequency", torch.float32, rows)
-            bits = (history.prompt.data_ptr(), history.output.data_ptr(),
-                    history.counts.data_ptr())
+            penalties = (*bits, n_slots, self._at(what, slots, "slots", i32, rows),
+                         self._at(what, repetition, "repetition", f32, rows),
+                         self._at(what, presence, "presence", f32, rows),
+                         self._at(what, frequency, "frequency", f32, rows))
         elif not (slots is repetition is presence is frequency is None):
             raise KernelError("logit_rules: penalties need a history")
+        biases = (0,) * 4
         if bias_start is not None:
-            self._fits(what, bias_start, "bias_start", torch.int32, rows + 1)
-            self._fits(what, bias_ids, "bias_ids", torch.int32, 0)
-            n_bias = bias_ids.shape[0]
-            self._fits(what, bias_values, "bias_values", torch.float32, n_bias)
-            if n_bias == 0:
-                bias_start = None
+            start = self._at(what, bias_start, "bias_start", i32, rows + 1)
+            ids = self._at(what, bias_ids, "bias_ids", i32, 0)
+            n = bias_ids.shape[0]
+            values = self._at(what, bias_values, "bias_values", f32, n)
+            if n:
+                biases = (start, ids, values, n)
         elif not (bias_ids is bias_values is None):
             raise KernelError("logit_rules: biases need bias_start")
+        masks = (0,) * 3
         if mask is not None:
-            _want(mask, "mask", torch.int32, 2)
-            self._drives(what, mask)
-            n_masks = mask.shape[0]
-            if mask.shape[1] != history_words(vocab):
-                raise KernelError(f"logit_rules: mask rows of {mask.shape[1]} words for {vocab} "
-                                  "logits")
-            self._fits(what, mask_row, "mask_row", torch.int32, rows)
-            if n_masks == 0:
-                mask = mask_row = None
+            at, n, words = self._matrix(what, mask, "mask", i32)
+            if words != history_words(vocab):
+                raise KernelError(f"logit_rules: mask rows of {words} words for {vocab} logits")
+            row = self._at(what, mask_row, "mask_row", i32, rows)
+            if n:
+                masks = (at, n, row)
         elif mask_row is not None:
             raise KernelError("logit_rules: mask_row needs a mask")
         if rows == 0:
             return
         self.launches += 1
-        _check(self.lib.hs_logit_rules(
-            a, b, rows, vocab, *bits, n_slots, _ptr(slots), _ptr(repetition),
-            _ptr(presence), _ptr(frequency), _ptr(bias_start), _ptr(bias_ids), _ptr(bias_values),
-            n_bias, _ptr(mask), n_masks, _ptr(mask_row), _ptr(self._status_of(logits)),
-            self._stream()), f"logit_rules(rows={rows},vocab={vocab})")
+        args = _RULES.pack(a, b, rows, vocab, *penalties, *biases, *masks,
+                           self._status_of(logits).data_ptr())
+        _check(self.lib.hs_logit_rules(args, self._stream()), what)
 
     # -- scores -------------------------------------------------------------------------------
     def token_logprobs(self, logprob, rank, logits, tokens, top_ids=None, top_logprobs=None):
@@ -2917,34 +2929,31 @@ class CudaOps:
         index), and with ``top_ids`` / ``top_logprobs`` ``[rows, n]`` the n tokens that come
         first in that order.  ``tokens[w] == -1``: no token (logprob NaN, rank -1).  A row of
         -inf alone has logprobs of -inf, one with a NaN or +inf has NaN."""
-        what = "token_logprobs"
-        _want(logits, "logits", torch.float32, 2)
-        self._drives(what, logits)
-        rows, vocab = logits.shape
-        self._fits(what, logprob, "logprob", torch.float32, rows)
-        self._fits(what, rank, "rank", torch.int32, rows)
-        self._fits(what, tokens, "tokens", torch.int32, rows)
+        what, i32, f32 = "token_logprobs", torch.int32, torch.float32
+        at, rows, vocab = self._matrix(what, logits, "logits", f32)
+        self._drives(what)
+        lp = self._at(what, logprob, "logprob", f32, rows)
+        rk = self._at(what, rank, "rank", i32, rows)
+        tokens_at = self._at(what, tokens, "tokens", i32, rows)
+        ids = lps = None
         top = 0
         if (top_ids is None) != (top_logprobs is None):
             raise KernelError("token_logprobs: top_ids and top_logprobs come together")
         if top_ids is not None:
-            _want(top_ids, "top_ids", torch.int32, 2)
-            _want(top_logprobs, "top_logprobs", torch.float32, 2)
-            self._drives(what, top_ids, top_logprobs)
-            top = top_ids.shape[1]
-            if top_ids.shape != top_logprobs.shape or top_ids.shape[0] < rows:
-                raise KernelError(f"token_logprobs: alternatives of shapes {tuple(top_ids.shape)} "
-                                  f"and {tuple(top_logprobs.shape)} for {rows} rows")
+            ids, *sizes = self._matrix(what, top_ids, "top_ids", i32)
+            lps, *others = self._matrix(what, top_logprobs, "top_logprobs", f32)
+            top = sizes[1]
+            if sizes != others or sizes[0] < rows:
+                raise KernelError(f"token_logprobs: alternatives of shapes {tuple(sizes)} and "
+                                  f"{tuple(others)} for {rows} rows")
             if top > min(MAX_ALTERNATIVES, vocab):
                 raise KernelError(f"token_logprobs: {top} alternatives; at most "
                                   f"{min(MAX_ALTERNATIVES, vocab)} of {vocab} tokens")
         if rows == 0:
             return
         self.launches += 1
-        _check(self.lib.hs_token_logprobs(
-            _ptr(logprob), _ptr(rank), _ptr(top_ids), _ptr(top_logprobs), top, _ptr(logits),
-            _ptr(tokens), rows, vocab, _ptr(self._status_of(logits)), self._stream()),
-            f"token_logprobs(rows={rows},vocab={vocab},top={top})")
+        _check(self.lib.hs_token_logprobs(lp, rk, ids, lps, top, at, tokens_at, rows, vocab,
+                                          self._status_of(logits).data_ptr(), self._stream()), what)
 
     # -- pages ----------------------------------------------------------------------------------
     def copy_pages(self, dst, src, dst_pages, src_pages, rows=None):
@@ -2954,21 +2963,24 @@ class CudaOps:
         lists are on the host.  Inside one pool no page may be written that is also read, and
         none twice anywhere: such lists are refused."""
         _want(dst, "dst", _FLOATS, 6)
-        _want(src, "src", dst.dtype, 6)
-        self._drives("copy_pages", dst, src)
-        if dst.shape[0] != src.shape[0] or dst.shape[2:] != src.shape[2:]:
-            raise KernelError(f"copy_pages: pools of shapes {tuple(dst.shape)} and "
-                              f"{tuple(src.shape)}")
-        one_pool = _shares_memory(dst, src)
-        to, of, part = page_lists(dst_pages, src_pages, rows, dst.shape[1], src.shape[1],
-                                  dst.shape[4], one_pool)
+        self._drives("copy_pages", dst)
+        entries, n_dst, planes, heads, page_rows, dim = dst.shape
+        n_src = n_dst
+        if src is not dst:
+            _want(src, "src", dst.dtype, 6)
+            self._drives("copy_pages", src)
+            n_src = src.shape[1]
+            if tuple(src.shape) != (entries, n_src, planes, heads, page_rows, dim):
+                raise KernelError(f"copy_pages: pools of shapes {tuple(dst.shape)} and "
+                                  f"{tuple(src.shape)}")
+        to, of, part = page_lists(dst_pages, src_pages, rows, n_dst, n_src, page_rows,
+                                  src is dst or _shares_memory(dst, src))
         n = len(to)
-        if n == 0:
+        if n == 0 or dst.numel() == 0:
             return
-        entries, _, planes, heads, page_rows, dim = dst.shape
         self.launches += -(-n // PAGE_LIST)
         _check(self.lib.hs_copy_pages(
             dst.data_ptr(), src.data_ptr(), n, to.buffer_info()[0], of.buffer_info()[0],
-            None if part is None else part.buffer_info()[0], entries, dst.shape[1], src.shape[1],
+            None if part is None else part.buffer_info()[0], entries, n_dst, n_src,
             planes * heads, page_rows, dim * dst.element_size(), self._stream()),
             f"copy_pages(n={n},entries={entries})")

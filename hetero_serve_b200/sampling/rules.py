@@ -21,12 +21,33 @@ from typing import Mapping, Sequence
 import numpy as np
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class LogitRules:
+    """The numbers of a request's rules; ValueError for numbers no request can mean."""
+
     repetition: float = 1.0
     presence: float = 0.0
     frequency: float = 0.0
     bias: Mapping[int, float] = field(default_factory=dict)
+    # the biases as arrays, as a step packs them
+    bias_ids: np.ndarray = field(init=False, repr=False)
+    bias_values: np.ndarray = field(init=False, repr=False)
+
+    def __post_init__(self):
+        if not (math.isfinite(self.repetition) and self.repetition > 0):
+            raise ValueError(f"repetition penalty {self.repetition} is not a positive number")
+        for name in ("presence", "frequency"):
+            if not math.isfinite(getattr(self, name)):
+                raise ValueError(f"{name} penalty {getattr(self, name)} is not a finite number")
+        for token, value in self.bias.items():
+            if isinstance(token, bool) or not isinstance(token, (int, np.integer)) \
+                    or not 0 <= token < 2 ** 31:
+                raise ValueError(f"bias of {token!r}, which is no token id")
+            if math.isnan(value) or value == math.inf:
+                raise ValueError(f"bias {value} of token {token}: neither a number nor -inf")
+        for name, kind, of in (("bias_ids", np.int32, self.bias.keys()),
+                               ("bias_values", np.float32, self.bias.values())):
+            object.__setattr__(self, name, np.fromiter(of, dtype=kind, count=len(self.bias)))
 
     @property
     def penalises(self) -> bool:
@@ -35,21 +56,12 @@ class LogitRules:
 
     @property
     def neutral(self) -> bool:
-        return not self.penalises and not self.bias
+        return not self.penalises and not len(self.bias_ids)
 
     def check(self, vocab: int | None = None) -> None:
-        """Raise ValueError for numbers no request can mean."""
-        if not (math.isfinite(self.repetition) and self.repetition > 0):
-            raise ValueError(f"repetition penalty {self.repetition} is not a positive number")
-        for name in ("presence", "frequency"):
-            if not math.isfinite(getattr(self, name)):
-                raise ValueError(f"{name} penalty {getattr(self, name)} is not a finite number")
-        for token, value in self.bias.items():
-            if isinstance(token, bool) or not isinstance(token, (int, np.integer)) or token < 0 \
-                    or (vocab is not None and token >= vocab):
-                raise ValueError(f"bias of token {token!r}, which the vocabulary does not have")
-            if math.isnan(value) or value == math.inf:
-                raise ValueError(f"bias {value} of token {token}: neither a number nor -inf")
+        """ValueError for a bias of a token the vocabulary does not have."""
+        if vocab is not None and len(self.bias_ids) and int(self.bias_ids.max()) >= vocab:
+            raise ValueError(f"bias of token {int(self.bias_ids.max())}: the vocabulary has {vocab}")
 
 
 def mask_words(allowed, vocab: int) -> np.ndarray | None:

@@ -352,7 +352,6 @@ def test_steps_refuse_rules_they_cannot_follow(tiny_models):
     for entry in (StepEntry("a", [1, 2], want=[1], rules=rules),                      # no history
                   StepEntry("a", [1, 2], want=[0], rules=rules, history=([1], [])),
                   StepEntry("a", [1, 2], want=[0, 1], allowed=words),
-                  StepEntry("a", [1, 2], want=[1], rules=LogitRules(repetition=0.0)),
                   StepEntry("a", [1, 2], want=[1], rules=LogitRules(bias={512: 1.0})),
                   StepEntry("a", [1, 2], want=[1], rules=rules, history=([512], [])),
                   StepEntry("a", [1, 2], want=[1], rules=rules, history=([1], [-1])),
@@ -369,6 +368,11 @@ def test_steps_refuse_rules_they_cannot_follow(tiny_models):
     rn.close("a")
     with pytest.raises(StepError, match="history"):                          # another request
         rn.step([StepEntry("b", [1], want=[0], rules=rules)], sample=True)
+    for bad in (dict(repetition=0.0), dict(bias={-1: 1.0}), dict(bias={2 ** 31: 1.0})):
+        with pytest.raises(ValueError):
+            LogitRules(**bad)
+    with pytest.raises(ValueError, match="alternatives"):
+        engine(tiny).score([1, 2], alternatives=33)
     with pytest.raises(ValueError, match="one answer"):
         engine(tiny).generate([[1, 2]], samples=2)
 
