@@ -199,6 +199,7 @@ class Scheduler:
         self.stats = SchedulerStats()
         self.pipeline = bool(pipeline)
         self.fork_fn = fork_fn or manager.fork
+        self._in_phase = True
         self._inflight: tuple[list[Planned], object] | None = None   # launched, tokens unread
         self._late_done: list[SequenceState] = []     # finished while a plan was being made
 
@@ -353,10 +354,15 @@ class Scheduler:
         mgr = self.manager
         planned: list[Planned] = []
         running = [s for s in self.active if s.state == SeqState.RUNNING][: self.max_batch]
+        # requests with grammars decode in the same steps (every second one, pipelined) instead of
+        # taking turns by halves; they sit out one step in a row for that, no more
+        self._in_phase = not self._in_phase or not any(
+            s.pending and s.request.grammar is not None for s in running)
         for seq in running:
-            if seq.pending and (self._ends_by_count(seq, seq.pending)
-                                or seq.request.grammar is not None):
-                continue                            # its token in flight is its last, or decides
+            if seq.pending and self._ends_by_count(seq, seq.pending):
+                continue                            # its token in flight is its last
+            if seq.request.grammar is not None and (seq.pending or not self._in_phase):
+                continue                            # its token in flight decides, or another's
             while seq.state == SeqState.RUNNING:    # else: preempted, or ended while we waited
                 try:
                     mgr.reserve(seq.req_id, seq.n_kv + 1)

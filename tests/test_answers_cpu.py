@@ -261,6 +261,32 @@ def test_the_rules_outlive_preemption(tiny_models):
         assert min(gaps) > 1e-4 and s.output_ids == want
 
 
+def test_grammars_decode_in_the_same_steps(tiny_models):
+    """Pipelined, requests with grammars whose prompts ended in different steps share their steps
+    all the same, and a plain request decodes in every one."""
+    tiny = tiny_models["tiny_b"]
+    eng = engine(tiny, pipeline=True, policy="mixed")
+    sizes = []
+    inner = eng.scheduler.step_fn
+
+    def counted(entries):
+        sizes.append([e.req_id for e in entries if e.want])
+        return inner(entries)
+    eng.scheduler.step_fn = counted
+    grammar = ac.Alternating(tiny.config["vocab_size"])
+    ruled = [eng.submit_nowait(Request(tiny.tokens(20, i), 12, stop_at_eos=False, grammar=grammar))
+             for i in range(4)]
+    plain = eng.submit_nowait(Request(tiny.tokens(5, 9), 40, stop_at_eos=False))
+    eng.run_until_done()
+    assert [len(s.output_ids) for s in ruled] == [12] * 4 and len(plain.output_ids) == 40
+    names = {s.req_id for s in ruled}
+    together = [len(names & set(step)) for step in sizes if len(step) > 0]
+    later = together[12:24]                       # (prompts end in the first few steps)
+    assert sorted(set(later)) == [0, 4], together
+    at = [i for i, step in enumerate(sizes) if plain.req_id in step]
+    assert at == list(range(at[0], at[0] + 40))
+
+
 def test_a_grammar_that_ends_the_answer(tiny_models):
     tiny = tiny_models["tiny_b"]
     eng = engine(tiny)
