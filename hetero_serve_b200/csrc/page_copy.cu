@@ -91,6 +91,10 @@ HS_EXPORT int hs_copy_pages(void* dst, const void* src, int n, const int* dst_li
     if (dst_list[i] < 0 || dst_list[i] >= dst_pages || src_list[i] < 0 || src_list[i] >= src_pages ||
         (rows && (rows[i] < 0 || rows[i] > page_rows)))
       return HS_ERR_ARGUMENT;
+  if (!rows) {                 // whole pages lie in one piece
+    row_bytes *= tiles * page_rows;
+    tiles = page_rows = 1;
+  }
   const uintptr_t bits = (uintptr_t)dst | (uintptr_t)src | (uintptr_t)row_bytes;
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
@@ -101,6 +105,7 @@ HS_EXPORT int hs_copy_pages(void* dst, const void* src, int n, const int* dst_li
           : hs::copy_pages<V, hs::PC_MANY>(dst, src, n, dst_list, src_list, rows, entries, dst_pages, \
                                            src_pages, tiles, page_rows, row_bytes, st)
   if (bits % 16 == 0) PC_GO(uint4);
+  else if (bits % 8 == 0) PC_GO(uint2);
   else if (bits % 4 == 0) PC_GO(uint32_t);
   else PC_GO(uint16_t);
 #undef PC_GO

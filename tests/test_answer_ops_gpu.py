@@ -430,6 +430,107 @@ def test_copies_move_bits(ops):
     assert flat[0].item() == bits[0].item()
 
 
+# -- large offsets, and what lies behind the rows ---------------------------------------------------
+
+
+def _room(gigabytes):
+    if torch.cuda.mem_get_info()[0] < gigabytes * 2 ** 30:
+        pytest.skip("not enough free device memory")
+
+
+def test_pages_behind_four_billion_numbers(ops):
+    _room(12)
+    pool = torch.empty(2, 34000, 2, 16, 32, 64, dtype=torch.bfloat16, device=DEV)     # 8.3 GiB
+    assert pool.numel() > 2 ** 32
+    pool[:, [5, 33999]] = torch.randn(2, 2, 2, 16, 32, 64, device=DEV).bfloat16()
+    ops.copy_pages(pool, pool, [33998, 7, 33997], [5, 33999, 33999], [32, 32, 11])
+    for e in range(2):
+        assert torch.equal(pool[e, 33998], pool[e, 5]) and torch.equal(pool[e, 7], pool[e, 33999])
+        assert torch.equal(pool[e, 33997, :, :, :11], pool[e, 33999, :, :, :11])
+    del pool
+    torch.cuda.empty_cache()
+
+
+def test_rows_behind_two_billion_logits(ops):
+    _room(24)
+    rows, vocab = 17000, 131101
+    x = torch.empty(rows, vocab, device=DEV)                                           # 8.3 GiB
+    assert x.numel() > 2 ** 31
+    x[-2:] = torch.randn(2, vocab, device=DEV)
+    keep = x[-2:].clone()
+    lp = torch.full((rows + 3,), 9.0, device=DEV)
+    rk = torch.full((rows + 3,), 9, dtype=torch.int32, device=DEV)
+    tokens = torch.full((rows,), -1, dtype=torch.int32, device=DEV)
+    tokens[-1] = int(keep[1].argmax())
+    ids = torch.full((rows + 1, 2), 9, dtype=torch.int32, device=DEV)
+    lps = torch.full((rows + 1, 2), 9.0, device=DEV)
+    ops.token_logprobs(lp, rk, x, tokens, ids, lps)
+    want = torch.log_softmax(keep[1].double(), 0)
+    assert rk[rows - 1].item() == 0 and abs(float(lp[rows - 1]) - float(want.max())) < 1e-4
+    assert torch.equal(ids[rows - 2:rows].long(), keep.topk(2, dim=1).indices)
+    assert bool((lp[rows:] == 9).all()) and bool((rk[rows:] == 9).all())               # left as they were
+    assert bool((ids[rows:] == 9).all()) and bool((lps[rows:] == 9).all())
+    history = history_of(17001, 1, DEV)            # (another vocabulary is refused)
+    start = torch.zeros(rows + 1, dtype=torch.int32, device=DEV)
+    start[rows] = 2
+    bias = dict(bias_start=start, bias_ids=ints([0, vocab - 1]).to(DEV),
+                bias_values=torch.tensor([1.0, -INF], device=DEV))
+    from hetero_serve_b200.kernels import KernelError
+    with pytest.raises(KernelError):
+        ops.logit_rules(x, x, history, tokens, lp, lp, lp, **bias)
+    ops.logit_rules(x, x, **bias)
+    keep[1, 0] += 1
+    keep[1, -1] = -INF
+    assert torch.equal(x[-2:], keep)
+    out = torch.empty_like(x)
+    ops.logit_rules(out, x, **bias)
+    keep[1, 0] += 1
+    assert torch.equal(out[-2:], keep)
+    del x, out
+    torch.cuda.empty_cache()
+    assert status(ops) == 0
+
+
+def test_a_record_behind_two_billion_counts(ops):
+    _room(12)
+    slots, vocab = 16400, 131101
+    h = history_of(slots, vocab, DEV)
+    assert h.counts.numel() > 2 ** 31
+    s = torch.tensor([slots - 1], dtype=torch.int32, device=DEV)
+    d = lambda x: ints(x).to(DEV)                                       # noqa: E731
+    ops.history_begin(h, s, d([vocab - 1, 3, 3]), d([0, 3]), d([1]))
+    ops.history_add(h, s, d([vocab - 1]))
+    assert h.counts[-1].nonzero().flatten().tolist() == [3, vocab - 1]
+    assert int(h.counts.sum()) == 3 and int((h.prompt != 0).sum()) == 1
+    x = torch.ones(1, vocab, device=DEV)
+    one = torch.ones(1, device=DEV)
+    ops.logit_rules(x, x, h, s, 2 * one, one, one)
+    assert x[0, 3].item() == 0.5 - 3 and x[0, -1].item() == 0.5 - 2 and x[0, 4].item() == 1
+    del h
+    torch.cuda.empty_cache()
+
+
+def test_tensors_elsewhere_are_refused(ops):
+    from hetero_serve_b200.kernels import KernelError
+    x = torch.zeros(2, 40, device=DEV)
+    one, i = torch.ones(2, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV)
+    with pytest.raises(KernelError):
+        ops.logit_rules(x.cpu(), x)
+    with pytest.raises(KernelError):
+        ops.logit_rules(x, x, history_of(2, 40), i, one, one, one)
+    with pytest.raises(KernelError):
+        ops.logit_rules(x, x, history_of(2, 40, DEV), i.cpu(), one, one, one)
+    with pytest.raises(KernelError):
+        ops.token_logprobs(one, i, x, i.cpu())
+    with pytest.raises(KernelError):
+        ops.token_logprobs(one, i[::2], x, i)
+    pool = torch.zeros(1, 4, 1, 1, 16, 8, device=DEV)
+    with pytest.raises(KernelError):
+        ops.copy_pages(pool, pool.cpu(), [0], [1])
+    with pytest.raises(KernelError):
+        ops.copy_pages(pool.cpu(), pool, [0], [1])
+
+
 # -- together, captured, on another stream --------------------------------------------------------
 
 
