@@ -68,8 +68,7 @@ logit_rules_kernel(const LogitRules a) {
   }
   if (tid == 0) {
     s_n = s_entries = 0;
-    if (blockIdx.x == 0 && (slot >= a.n_slots || mrow >= a.n_masks) &&
-        ((a.slots && slot >= a.n_slots) || (a.mask && mrow >= a.n_masks)))
+    if (blockIdx.x == 0 && (slot >= a.n_slots || mrow >= a.n_masks))      // (without tables: -1 >= 0)
       atomicOr(a.status, HS_STATUS_BAD_ROW);
   }
   const size_t first = (size_t)w * a.vocab + lo;

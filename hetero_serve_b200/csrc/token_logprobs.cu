@@ -20,7 +20,6 @@ namespace hs {
 
 constexpr int TL_TOP = 32;                // a warp's lanes hold the alternatives, in order
 constexpr int TL_GROUPS = 32;             // of threads, whose maxima give the bound
-constexpr int TL_INFLIGHT = 4;            // 16-byte loads a thread has under way
 constexpr int TL_CAND = 1024;             // logits looked at again at a time
 constexpr int TL_FEW = 256;               // ... that are put in order by counting
 
@@ -139,7 +138,10 @@ __global__ void __launch_bounds__(THREADS)
 token_logprobs_kernel(float* __restrict__ logprob, int* __restrict__ rank, int* __restrict__ top_ids,
                       float* __restrict__ top_logprobs, int top, const float* __restrict__ logits,
                       const int* __restrict__ tokens, int vocab, int* status) {
-  constexpr int WARPS = THREADS / 32, STEP = TL_INFLIGHT * THREADS;
+  // 16-byte loads a thread has under way: four, where the rows fill the SMs three, which leaves an SM
+  // the registers for a fourth block (512 x 50,257: 19.8 and 16.5 us, 2,048 x 50,257: 68.3 and 67.6)
+  constexpr int INFLIGHT = BLOCKS == 1 && THREADS == 512 ? 3 : 4;
+  constexpr int WARPS = THREADS / 32, STEP = INFLIGHT * THREADS;
   static_assert(THREADS >= 2 * TL_GROUPS && THREADS >= BLOCKS * TL_TOP && BLOCKS * TL_TOP <= TL_CAND, "");
   __shared__ TlSum s_sum[WARPS];
   __shared__ int s_before[WARPS];
@@ -182,15 +184,15 @@ token_logprobs_kernel(float* __restrict__ logprob, int* __restrict__ rank, int* 
   }
   float m_pieces = -INFINITY;             // the largest in the thread's pieces
   auto chunk = [&](int at, bool whole) {  // pieces at + tid, + THREADS, ...
-    float4 f[TL_INFLIGHT];
+    float4 f[INFLIGHT];
 #pragma unroll
-    for (int i = 0; i < TL_INFLIGHT; ++i) {
+    for (int i = 0; i < INFLIGHT; ++i) {
       f[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       if (whole || at + tid + i * THREADS < p1) f[i] = row[at + tid + i * THREADS];
     }
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < TL_INFLIGHT; ++i)
+    for (int i = 0; i < INFLIGHT; ++i)
       m = fmaxf(fmaxf(fmaxf(m, f[i].x), f[i].y), fmaxf(f[i].z, f[i].w));
     m_pieces = fmaxf(m_pieces, m);
     if (m > own.m) {
@@ -201,7 +203,7 @@ token_logprobs_kernel(float* __restrict__ logprob, int* __restrict__ rank, int* 
     const tl_pair ref2 = tl_two(ref, ref), scale2 = tl_two(TL_LOG2E, TL_LOG2E);
     tl_pair sum2 = tl_two(own.s, 0.f);
 #pragma unroll
-    for (int i = 0; i < TL_INFLIGHT; ++i) {
+    for (int i = 0; i < INFLIGHT; ++i) {
       const float2 a = tl_apart(tl_mul(tl_add(tl_two(f[i].x, f[i].y), ref2), scale2));
       const float2 b = tl_apart(tl_mul(tl_add(tl_two(f[i].z, f[i].w), ref2), scale2));
       sum2 = tl_add(sum2, tl_two(tl_exp2(a.x), tl_exp2(a.y)));
@@ -211,7 +213,7 @@ token_logprobs_kernel(float* __restrict__ logprob, int* __restrict__ rank, int* 
     own.s = sum.x + sum.y;
     if (by_key) {
 #pragma unroll
-      for (int i = 0; i < TL_INFLIGHT; ++i) {
+      for (int i = 0; i < INFLIGHT; ++i) {
         const int p = at + tid + i * THREADS, v = head + 4 * p;
         if (p < p1)
           before += (tl_key(f[i].x, v) > mine) + (tl_key(f[i].y, v + 1) > mine) +
@@ -219,7 +221,7 @@ token_logprobs_kernel(float* __restrict__ logprob, int* __restrict__ rank, int* 
       }
     } else if (m > below) {               // (most often nothing here stands before the token)
 #pragma unroll
-      for (int i = 0; i < TL_INFLIGHT; ++i) {
+      for (int i = 0; i < INFLIGHT; ++i) {
         const int v = head + 4 * (at + tid + i * THREADS);
         before += (f[i].x > (v < t ? below : xt)) + (f[i].y > (v + 1 < t ? below : xt)) +
                   (f[i].z > (v + 2 < t ? below : xt)) + (f[i].w > (v + 3 < t ? below : xt));
