@@ -103,7 +103,8 @@ class LLMEngine:
         return out
 
     def submit(self, request: Request) -> RequestRecord:
-        """Run until this request has finished (others in flight advance too)."""
+        """Run until this request has finished (others in flight advance too; of several samples
+        this is the first: see :meth:`submit_samples`)."""
         seq = self.submit_nowait(request)
         while seq.state != "done":
             self.step()

@@ -405,13 +405,15 @@ class Scheduler:
 
     def _masks(self, planned: list[Planned]) -> dict:
         """What the planned requests' grammars allow next, packed, by request.  A request whose
-        grammar allows nothing any more ends here."""
+        grammar allows nothing any more (that its biases do not rule out) ends here."""
         masks = {}
         for p in planned:
             grammar = p.seq.request.grammar
             if grammar is None or not p.samples:
                 continue
             words = mask_words(grammar.allowed(tuple(p.seq.output_ids)), self.vocab_size)
+            if words is not None and p.seq.rules is not None and len(p.seq.rules.ruled_out):
+                words &= ~mask_words(p.seq.rules.ruled_out, self.vocab_size)
             if words is not None and not words.any():
                 p.seq.finish_reason = "grammar"
                 self._finish(p.seq, self.clock())

@@ -443,14 +443,15 @@ class Runner:
                 rows += [t.view(torch.float32) for t in self.history.tensors()]
                 self._recorded.add(to)
             for t in rows:                     # a row a slot: a page of one row
-                view = t.view(1, t.shape[0], 1, 1, 1, -1)
-                self.ops.copy_pages(view, view, [to], [of])
+                if t.numel():                  # (a state may be empty: a convolution of one tap)
+                    view = t.view(1, t.shape[0], 1, 1, 1, -1)
+                    self.ops.copy_pages(view, view, [to], [of])
 
     def resize_cache(self, num_pages: int) -> None:
         """Give the page groups pools of the size ``num_pages`` stands for when a runner is made.
         Live requests keep their pages (moved to the lowest numbers of the new pools), published
         prefixes as far as they fit.  Raises :class:`OutOfPages` with nothing changed when the
-        live requests' pages do not fit; both pools of a group exist while its pages move.  The
+        live requests' pages do not fit; the old and new pools exist side by side meanwhile.  The
         longest request the runner takes (``max_positions``) stays what it was."""
         mgr, model = self.manager, self.model
         sizes = [-(-num_pages // g.stride) + mgr.max_requests if g.stride > 1 else num_pages

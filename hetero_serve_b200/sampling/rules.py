@@ -7,9 +7,10 @@ generated c > 0 times loses ``frequency * c + presence``; a biased token gains i
 that the grammar rules out becomes -inf.
 
 A *grammar* is any object with ``allowed(output_ids)``: asked before every token with the tokens
-generated so far, it says which may come next — ``None`` (any), a packed mask
-(``ceil(vocab / 32)`` 32-bit words, bit v % 32 of word v // 32), truth values over the
-vocabulary, or token ids.  An answer that allows nothing ends the request.
+generated so far, it says which may come next — ``None`` (any), a packed mask (an array of
+``ceil(vocab / 32)`` 32-bit words, bit v % 32 of word v // 32), an array of truth values over the
+vocabulary, or token ids (anything else that yields whole numbers; 32-bit arrays are masks).  An
+answer that allows nothing ends the request.
 """
 
 from __future__ import annotations
@@ -48,6 +49,11 @@ class LogitRules:
         for name, kind, of in (("bias_ids", np.int32, self.bias.keys()),
                                ("bias_values", np.float32, self.bias.values())):
             object.__setattr__(self, name, np.fromiter(of, dtype=kind, count=len(self.bias)))
+
+    @property
+    def ruled_out(self) -> list[int]:
+        """The tokens whose bias is -inf."""
+        return self.bias_ids[np.isneginf(self.bias_values)].tolist()
 
     @property
     def penalises(self) -> bool:

@@ -269,6 +269,28 @@ def test_counts_above_the_exact_integers_of_float32(ops):
     check_rules(ops, s)
 
 
+@pytest.mark.parametrize("vocab", [40, 5003, 50257])
+def test_sampling_stays_within_what_the_rules_leave(ops, vocab):
+    """Every sampler over rows of which one, two or five tokens are left, with k below and above."""
+    rows = 24
+    gen = torch.Generator().manual_seed(vocab)
+    left = [torch.randperm(vocab, generator=gen)[:(1, 2, 5)[r % 3]] for r in range(rows)]
+    flags = torch.zeros(rows, vocab, dtype=torch.bool)
+    for r, ids in enumerate(left):
+        flags[r, ids] = True
+    x = (torch.randn(rows, vocab, generator=gen) * 4).to(DEV)
+    out = torch.empty_like(x)
+    row = torch.arange(rows, dtype=torch.int32, device=DEV)
+    ops.logit_rules(out, x, mask=pack(flags).to(DEV), mask_row=row)
+    tokens, zero = torch.empty_like(row), torch.zeros_like(row)
+    for k in (0, 1, 3, 30):
+        for temperature in (0.0, 0.7, 3.0):
+            for position in range(4):
+                ops.sample(tokens, out, torch.full((rows,), temperature, device=DEV), zero + k, row, zero,
+                           zero + position)
+                assert all(t in ids.tolist() for t, ids in zip(tokens.tolist(), left)), (k, temperature)
+
+
 # -- log-probabilities --------------------------------------------------------------------------
 
 

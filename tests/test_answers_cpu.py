@@ -296,6 +296,10 @@ def test_a_grammar_that_ends_the_answer(tiny_models):
     closed = eng.submit(Request(tiny.tokens(9, 1), 10, grammar=OneOf(choices, end=999)))
     assert closed.output_ids == [*open_end.output_ids, 999] and closed.finish_reason == "eos"
 
+    banned = eng.submit(Request(tiny.tokens(9, 1), 10, grammar=OneOf([[4, 5], [6]]),
+                                logit_bias={5: -math.inf, 6: -math.inf}))
+    assert banned.output_ids == [4] and banned.finish_reason == "grammar"
+
     class Nothing:
         def allowed(self, output):
             return []
@@ -401,6 +405,30 @@ def test_steps_refuse_rules_they_cannot_follow(tiny_models):
         engine(tiny).score([1, 2], alternatives=33)
     with pytest.raises(ValueError, match="one answer"):
         engine(tiny).generate([[1, 2]], samples=2)
+
+
+@pytest.mark.parametrize("family", ["pedorax", "putelix", "roritar", "mafuzen", "pivinex", "nukodra"])
+@pytest.mark.parametrize("name", ["case_a", "case_b"])
+def test_forks_in_every_architecture(request, family, name):
+    """Windows, chunks, companion rows, shared latents, states, empty ones among them: a fork goes on
+    as a request of its own that was fed the same tokens, bit for bit."""
+    from hetero_serve_b200.engine import Runner
+    from hetero_serve_b200.engine.loading import load_model
+    case = request.getfixturevalue(f"{family}_cases")[name]
+    vocab, n = case.config["vocab"], 23
+    t = case.tokens(n + 2, 5)
+    model, _ = load_model(case.dir, "float32", "cpu")
+    rn = Runner(model, num_pages=48, page_size=16, max_requests=4, dtype=torch.float32, device="cpu",
+                ops=PlainAnswerOps())
+    rn.step([StepEntry("a", t[:n])])
+    rn.fork("a", "b")
+    rn.step([StepEntry("alone", t[:n])])
+    for i in range(n, n + 2):
+        other = [(t[i] + 1) % vocab]
+        res = rn.step([StepEntry("a", [t[i]], want=[0]), StepEntry("b", other, want=[0]),
+                       StepEntry("alone", other, want=[0])])
+        assert torch.equal(res.logits[1], res.logits[2]) and not torch.equal(res.logits[0], res.logits[1])
+    rn.manager.check()
 
 
 def test_a_fork_goes_on_where_its_parent_stood(tiny_models):

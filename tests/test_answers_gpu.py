@@ -102,13 +102,14 @@ def test_samples_equal_requests_of_their_own(tiny_models, dtype, graphs):
                 assert abs(record.cumulative_logprob - want.cumulative_logprob) < 1e-3
 
 
-def test_a_choice_and_plain_requests_side_by_side(tiny_models):
+@pytest.mark.parametrize("top_k", [0, 2, 40])
+def test_a_choice_and_plain_requests_side_by_side(tiny_models, top_k):
     tiny = tiny_models["tiny_b"]
     eng = engine(tiny.dir, policy="mixed")
     choices = [[4, 5, 6], [4, 9], [7, 8, 9, 10]]
     beside = [eng.submit_nowait(Request(tiny.tokens(20 + i, i), 12, stop_at_eos=False))
               for i in range(3)]
-    chosen = [eng.submit_nowait(Request(tiny.tokens(9 + i, 5 + i), 10, 0.8, seed=i,
+    chosen = [eng.submit_nowait(Request(tiny.tokens(9 + i, 5 + i), 10, 0.8, top_k, seed=i,
                                         grammar=OneOf(choices, end=999))) for i in range(3)]
     eng.run_until_done()
     for s in chosen:
@@ -159,6 +160,7 @@ def _models(request):
     for family in ("pedorax", "putelix", "roritar", "mafuzen", "pivinex", "nukodra"):
         cases = request.getfixturevalue(f"{family}_cases")
         yield family, cases["case_a"]
+        yield family, cases["case_b"]
         if family in ("putelix", "nukodra"):
             yield family, cases["case_d"]
 
