@@ -5,6 +5,11 @@
 // page stay as they were.  dst and src may be one pool: the caller sees to it that no page is
 // written twice, nor written and read.  The list travels as a kernel argument, so that no copy of
 // it has to be made on the device, and kept there, before the launch.
+//
+// Bound by the bytes, each read and written once: 2,500 pages of 12 entries (1.47 GB one way) take 454 us,
+// 6.5 TB/s, the rate of a plain copy.  A few pages are bound by the launch: 7 half pages of 24
+// entries 3.4 us.  48 pages of 24 entries in float32, half filled, took 25 us as a block a page and
+// entry and 18 as blocks of four rounds of four 16-byte loads a thread (mostly from the L2).
 #include "common.cuh"
 
 namespace hs {

@@ -14,6 +14,13 @@
 // equal for that (a row of zeros, of -inf), or NaNs leave too few, the threads' largest logits are
 // ordered with their indices instead, which bounds what is looked at whatever the values are.
 // A row is shared by the blocks of a cluster where there are few rows.
+//
+// Bound by the bytes of the logits where there are many rows (2,048 x 50,257 without alternatives:
+// 69 us in a graph, 63 at the copy rate; the exponentials' pipe is half busy), by the chain of barriers
+// behind the pass where there are few (one row: 3.8 us, 6.0 with 5 alternatives; 64 rows with 20: 9.6).
+// Two numbers an instruction (add and mul on pairs), 2^x without the scaling of results below 2^-126,
+// and counting before x_t only where a chunk holds something larger took the pass from 24
+// instructions a logit to 11 (82 -> 69 us).
 #include "common.cuh"
 
 namespace hs {

@@ -470,6 +470,7 @@ class CudaOps:
         # One object drives one device.  Its kernels are launched on that device's current
         # stream, so the device must be current while they are (the runner sees to it).
         self.device = dev
+        self._index = dev.index
         self.lib = load_library()
         self.launches = 0          # kernels launched through this object (graph captures count once)
         self.tensor_cores = True   # linears on tcgen05 (False: CUDA cores, float32 as chains of FMAs; for tests)
@@ -530,7 +531,7 @@ class CudaOps:
 
     def _stream(self):
         # (the stream's handle without a Stream object around it, which costs 2 us a launch)
-        return torch._C._cuda_getCurrentRawStream(self.device.index)
+        return torch._C._cuda_getCurrentRawStream(self._index)
 
     # -- kernels that parts bring themselves -------------------------------------------
     def stream(self) -> int:
@@ -2788,7 +2789,7 @@ class CudaOps:
         is refused."""
         try:
             if (t.dtype is dtype and t.numel() >= rows and t.dim() == 1
-                    and t.get_device() == self.device.index and t.is_contiguous()):
+                    and t.get_device() == self._index and t.is_contiguous()):
                 return t.data_ptr()
         except AttributeError:
             pass
@@ -2801,7 +2802,7 @@ class CudaOps:
     def _matrix(self, what, t, name, dtype):
         """Where a matrix lies on this object's device, and its sizes."""
         try:
-            if (t.dtype is dtype and t.dim() == 2 and t.get_device() == self.device.index
+            if (t.dtype is dtype and t.dim() == 2 and t.get_device() == self._index
                     and t.is_contiguous()):
                 return t.data_ptr(), *t.shape
         except AttributeError:
@@ -2813,10 +2814,10 @@ class CudaOps:
     def _drives(self, what, *tensors):
         """Kernels run on this object's device, which has to be the current one."""
         for t in tensors:
-            if t.device != self.device:
+            if t.get_device() != self._index:
                 raise KernelError(f"{what}: a tensor on {t.device}; these kernels drive "
                                   f"{self.device}")
-        if torch.cuda.current_device() != self.device.index:
+        if torch._C._cuda_getDevice() != self._index:
             raise KernelError(f"{what}: device {torch.cuda.current_device()} is current; these "
                               f"kernels drive {self.device}")
 

@@ -29,7 +29,7 @@ def ops(monkeypatch):
                         lambda t, name, dtype=None, dim=None, cuda=True, _w=ops_module._want:
                         _w(t, name, dtype, dim, False))
     o = CudaOps.__new__(CudaOps)
-    o.device, o.lib, o.launches = torch.device("cpu"), NoLibrary(), 0
+    o.device, o._index, o.lib, o.launches = torch.device("cpu"), -1, NoLibrary(), 0
     o.status = torch.zeros(1, dtype=torch.int32)
     monkeypatch.setattr(CudaOps, "_stream", lambda self: 0)
     monkeypatch.setattr(CudaOps, "_drives", lambda self, what, *tensors: None)
