@@ -16,7 +16,7 @@
 // A row is shared by the blocks of a cluster where there are few rows.
 //
 // Bound by the bytes of the logits where there are many rows (2,048 x 50,257 without alternatives:
-// 69 us in a graph, 63 at the copy rate; the exponentials' pipe is half busy), by the chain of barriers
+// 66 us in a graph, 63 at the copy rate; the exponentials' pipe is half busy), by the chain of barriers
 // behind the pass where there are few (one row: 3.8 us, 6.0 with 5 alternatives; 64 rows with 20: 9.6).
 // Two numbers an instruction (add and mul on pairs), 2^x without the scaling of results below 2^-126,
 // and counting before x_t only where a chunk holds something larger took the pass from 24
@@ -140,14 +140,12 @@ __device__ __forceinline__ T tl_remote(const T* p, int rank) {
   }
 }
 
-template <int THREADS, int BLOCKS>
+// INFLIGHT: 16-byte loads a thread has under way
+template <int THREADS, int BLOCKS, int INFLIGHT>
 __global__ void __launch_bounds__(THREADS)
 token_logprobs_kernel(float* __restrict__ logprob, int* __restrict__ rank, int* __restrict__ top_ids,
                       float* __restrict__ top_logprobs, int top, const float* __restrict__ logits,
                       const int* __restrict__ tokens, int vocab, int* status) {
-  // 16-byte loads a thread has under way: four, where the rows fill the SMs three, which leaves an SM
-  // the registers for a fourth block (512 x 50,257: 19.8 and 16.5 us, 2,048 x 50,257: 68.3 and 67.6)
-  constexpr int INFLIGHT = BLOCKS == 1 && THREADS == 512 ? 3 : 4;
   constexpr int WARPS = THREADS / 32, STEP = INFLIGHT * THREADS;
   static_assert(THREADS >= 2 * TL_GROUPS && THREADS >= BLOCKS * TL_TOP && BLOCKS * TL_TOP <= TL_CAND, "");
   __shared__ TlSum s_sum[WARPS];
@@ -429,7 +427,7 @@ token_logprobs_kernel(float* __restrict__ logprob, int* __restrict__ rank, int* 
   }
 }
 
-template <int THREADS, int BLOCKS>
+template <int THREADS, int BLOCKS, int INFLIGHT>
 cudaError_t token_logprobs(float* logprob, int* rank, int* top_ids, float* top_logprobs, int top,
                            const float* logits, const int* tokens, int rows, int vocab, int* status,
                            cudaStream_t stream) {
@@ -454,7 +452,7 @@ cudaError_t token_logprobs(float* logprob, int* rank, int* top_ids, float* top_l
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<THREADS, BLOCKS>, logprob, rank, top_ids,
+  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<THREADS, BLOCKS, INFLIGHT>, logprob, rank, top_ids,
                             top_logprobs, top, logits, tokens, vocab, status);
 }
 
@@ -475,17 +473,21 @@ HS_EXPORT int hs_token_logprobs(float* logprob, int* rank, int* top_ids, float* 
   // only where it is long: us in a graph, one block against the choice, with 20 alternatives:
   // 1 x 50,257 8.3 and 7.0, 64 x 50,257 8.8 and 9.1 (18.5 and 16.4 with the logits out of the L2),
   // 128 x 50,257 11.7 and 10.6, 32 x 131,072 13.7 and 10.0; 32 x 16,384 5.6 and over 2 blocks 6.6.
-  // Short rows take half the threads (128 x 4,096: 4.8, with 512 threads 6.1).
+  // Short rows take half the threads (128 x 4,096: 4.8, with 512 threads 6.1), and so do long ones that
+  // want no alternatives and fill the SMs (600 x 50,257: 26 and 28, 2,048 x 50,257: 66 and 69).  Rows that
+  // fill the SMs have three loads a thread under way, which leaves an SM the registers for another
+  // block (512 x 50,257 with four: 19.8, with three 16.5).
   const int blocks = vocab <= 24576 ? 1 : rows <= 37 ? 8 : rows <= 74 ? 4 : rows <= 148 ? 2 : 1;
   cudaError_t e;
-#define TL_GO(THREADS, BLOCKS)                                                                      \
-  e = hs::token_logprobs<THREADS, BLOCKS>(logprob, rank, top_ids, top_logprobs, top, logits, tokens, \
-                                          rows, vocab, status, st)
-  if (blocks == 8) TL_GO(512, 8);
-  else if (blocks == 4) TL_GO(512, 4);
-  else if (blocks == 2) TL_GO(512, 2);
-  else if (vocab <= 8192) TL_GO(256, 1);
-  else TL_GO(512, 1);
+#define TL_GO(THREADS, BLOCKS, INFLIGHT)                                                              \
+  e = hs::token_logprobs<THREADS, BLOCKS, INFLIGHT>(logprob, rank, top_ids, top_logprobs, top, logits, \
+                                                    tokens, rows, vocab, status, st)
+  if (blocks == 8) TL_GO(512, 8, 4);
+  else if (blocks == 4) TL_GO(512, 4, 4);
+  else if (blocks == 2) TL_GO(512, 2, 4);
+  else if (vocab <= 8192) TL_GO(256, 1, 4);
+  else if (top == 0 && rows > 148) TL_GO(256, 1, 3);
+  else TL_GO(512, 1, 3);
 #undef TL_GO
   return e == cudaSuccess ? HS_OK : (int)e;
 }

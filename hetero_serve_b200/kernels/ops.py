@@ -2836,7 +2836,7 @@ class CudaOps:
         the first ``n_prompt[k]`` of which are its prompt's and the others generated.  What the
         slot held before is gone; other slots stay.  A slot below zero is skipped; of two rows
         of one slot the last counts.  Token ids outside the vocabulary are left out and
-        reported in the status word."""
+        reported in the status word, offsets outside ``tokens`` cut to it.  At most 65,535 rows."""
         what, i32 = "history_begin", torch.int32
         record = self._history(what, history)
         at = self._at(what, slots, "slots", i32, 0)
@@ -2844,6 +2844,8 @@ class CudaOps:
         tokens_at = self._at(what, tokens, "tokens", i32, 0)
         prompt_at = self._at(what, n_prompt, "n_prompt", i32, rows)
         start_at = self._at(what, start, "start", i32, rows + 1)
+        if rows == 0:
+            return
         self.launches += 1
         _check(self.lib.hs_history_begin(
             *record, at, rows, tokens_at, tokens.shape[0], start_at, prompt_at,
@@ -2857,6 +2859,8 @@ class CudaOps:
         at = self._at(what, slots, "slots", torch.int32, 0)
         rows = slots.shape[0]
         tokens_at = self._at(what, tokens, "tokens", torch.int32, rows)
+        if rows == 0:
+            return
         self.launches += 1
         _check(self.lib.hs_history_add(output, counts, n_slots, vocab, at, tokens_at, rows,
                                        self._status_of(slots).data_ptr(), self._stream()), what)
@@ -2876,7 +2880,8 @@ class CudaOps:
           no mask).
 
         The arithmetic on a token is done in 64 bits and rounded once.  Ids, records and masks
-        outside their tables are left out and reported in the status word."""
+        outside their tables are left out and reported in the status word; a row that is ruled
+        out throughout is -inf throughout.  At most 65,535 rows."""
         what, i32, f32 = "logit_rules", torch.int32, torch.float32
         b, rows, vocab = self._matrix(what, logits, "logits", f32)
         a, *sizes = self._matrix(what, out, "out", f32)
@@ -2911,9 +2916,9 @@ class CudaOps:
             at, n, words = self._matrix(what, mask, "mask", i32)
             if words != history_words(vocab):
                 raise KernelError(f"logit_rules: mask rows of {words} words for {vocab} logits")
-            row = self._at(what, mask_row, "mask_row", i32, rows)
-            if n:
-                masks = (at, n, row)
+            if n == 0:
+                raise KernelError("logit_rules: a table of no masks")
+            masks = (at, n, self._at(what, mask_row, "mask_row", i32, rows))
         elif mask_row is not None:
             raise KernelError("logit_rules: mask_row needs a mask")
         if rows == 0:
@@ -2961,7 +2966,8 @@ class CudaOps:
         """``dst[:, dst_pages[i], :, :, :rows[i]] = src[:, src_pages[i], :, :, :rows[i]]`` for
         every i (``rows`` None: whole pages), for pools ``[entries, pages, planes, kv_heads,
         page_size, head_dim]`` of one type that differ in their number of pages at most.  The
-        lists are on the host.  Inside one pool no page may be written that is also read, and
+        lists are on the host and read before this returns (a captured call replays with the lists
+        it was captured with).  Inside one pool no page may be written that is also read, and
         none twice anywhere: such lists are refused."""
         _want(dst, "dst", _FLOATS, 6)
         self._drives("copy_pages", dst)

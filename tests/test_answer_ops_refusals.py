@@ -112,7 +112,7 @@ def test_rules_refuse_what_does_not_fit(ops):
            dict(bias_start=i32(4), bias_ids=i32(2), bias_values=torch.zeros(1)),
            dict(bias_start=i32(4), bias_ids=i32(2)), dict(bias_ids=i32(2)),
            dict(mask=i32(2, 3), mask_row=i32(3)), dict(mask=i32(2, 4), mask_row=i32(2)),
-           dict(mask=i32(2, 4)), dict(mask_row=i32(3))]
+           dict(mask=i32(2, 4)), dict(mask_row=i32(3)), dict(mask=i32(0, 4), mask_row=i32(3))]
     for kw in bad:
         with pytest.raises(KernelError):
             ops.logit_rules(out, x, **kw)
@@ -141,6 +141,8 @@ def test_histories_and_scores_refuse_what_does_not_fit(ops):
             ops.history_begin(h, **{**args, **kw})
     with pytest.raises(KernelError):
         ops.history_add(h, i32(3), i32(2))
+    ops.history_begin(h, i32(0), i32(0), i32(1), i32(0))
+    ops.history_add(h, i32(0), i32(0))
     x, lp, rk = torch.zeros(3, 30), torch.zeros(3), i32(3)
     for args, kw in (((lp[:2], rk, x, i32(3)), {}), ((lp, rk, x, i32(2)), {}),
                      ((lp, lp, x, i32(3)), {}), ((lp, rk, x.double(), i32(3)), {}),

@@ -388,6 +388,7 @@ def test_steps_refuse_rules_they_cannot_follow(tiny_models):
                   StepEntry("a", [1, 2], want=[1], allowed=words[:15]),
                   StepEntry("a", [1, 2], want=[1], allowed=words.astype(np.int64)),
                   StepEntry("a", [1, 2], want=[1], allowed=[1, 2]),
+                  StepEntry("a", [1, 2], want=[1], allowed=words * 0),
                   StepEntry("a", [1, 2], want=[1], logprobs=33),
                   StepEntry("a", [1, 2], want=[1], logprobs=-1)):
         with pytest.raises(StepError):
