@@ -3,6 +3,7 @@ without a GPU: manager and scheduler alone, then the engine over the plain twins
 against an oracle over the plain model's logits."""
 
 import math
+import random
 
 import numpy as np
 import pytest
@@ -446,3 +447,17 @@ def test_a_fork_goes_on_where_its_parent_stood(tiny_models):
         a, b = res.tokens_host()
         assert a == b and torch.equal(res.logits[0], res.logits[1])
     rn.manager.check()
+
+
+@pytest.mark.parametrize("seed", (0, 3, 4, 11))
+def test_everything_at_once_depends_on_no_engine_setting(tiny_models, seed):
+    """Penalties, biases, grammars, samples and scores of requests that come and go: batches, budgets,
+    pipelining, prefix reuse, preemption and the cache's size change no answer."""
+    tiny = tiny_models["tiny_a"]
+    requests = ac.any_requests(random.Random(seed), tiny.config["vocab_size"])
+    answers = [ac.run_through(engine(tiny, **options), requests, random.Random(seed + 100))
+               for options in ac.ENGINES]
+    first, scores = answers[0]
+    for other, others in answers[1:]:
+        # (a row's sum is taken in another order where it lies on other 16-byte borders)
+        assert other == first and torch.allclose(others, scores, rtol=0, atol=1e-5)

@@ -3,6 +3,7 @@ through the engine on the GPU: captured and launched one by one, pipelined or no
 architecture's cache and state."""
 
 import math
+import random
 
 import pytest
 import torch
@@ -225,3 +226,17 @@ def test_command_line_gives_scored_samples():
     for rec in lines[:6]:
         assert len(rec["output_ids"]) == 4 == len(rec["logprobs"]) and 5 not in rec["output_ids"]
         assert all(len(t) == 2 for t in rec["top_logprobs"])
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_everything_at_once_depends_on_no_engine_setting(tiny_models, seed):
+    """Penalties, biases, grammars, samples and scores of requests that come and go: batches, budgets,
+    pipelining, prefix reuse, preemption and the cache's size change no answer."""
+    tiny = tiny_models["tiny_a"]
+    requests = ac.any_requests(random.Random(seed), tiny.config["vocab_size"])
+    answers = [ac.run_through(engine(tiny.dir, **options), requests, random.Random(seed + 100))
+               for options in ac.ENGINES]
+    first, scores = answers[0]
+    for other, others in answers[1:]:
+        # (a row's sum is taken in another order where it lies on other 16-byte borders)
+        assert other == first and torch.allclose(others, scores, rtol=0, atol=1e-5)
