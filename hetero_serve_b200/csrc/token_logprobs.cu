@@ -469,15 +469,18 @@ HS_EXPORT int hs_token_logprobs(float* logprob, int* rank, int* top_ids, float* 
   if (rows <= 0) return HS_OK;
   if (rows > (1 << 27) || vocab > 0x7ffffff0) return HS_ERR_UNSUPPORTED;
   cudaStream_t st = (cudaStream_t)stream;
-  // A row over 8, 4 or 2 blocks of 512 threads while that gives every SM two blocks or fewer, and
-  // only where it is long: us in a graph, one block against the choice, with 20 alternatives:
-  // 1 x 50,257 8.3 and 7.0, 64 x 50,257 8.8 and 9.1 (18.5 and 16.4 with the logits out of the L2),
-  // 128 x 50,257 11.7 and 10.6, 32 x 131,072 13.7 and 10.0; 32 x 16,384 5.6 and over 2 blocks 6.6.
-  // Short rows take half the threads (128 x 4,096: 4.8, with 512 threads 6.1), and so do long ones that
-  // want no alternatives and fill the SMs (600 x 50,257: 26 and 28, 2,048 x 50,257: 66 and 69).  Rows that
-  // fill the SMs have three loads a thread under way, which leaves an SM the registers for another
-  // block (512 x 50,257 with four: 19.8, with three 16.5).
-  const int blocks = vocab <= 24576 ? 1 : rows <= 37 ? 8 : rows <= 74 ? 4 : rows <= 148 ? 2 : 1;
+  // A long row over 8, 4 or 2 blocks of 512 threads, as many as find room at once: two such blocks fit an
+  // SM, and a cluster of 8 or 4 needs its SMs in one group of the chip, so that 35 clusters of 8 take
+  // turns (us in a graph with 20 alternatives, over 8, 4, 2 and 1 blocks: 1 x 50,257 7.1, 6.7, 7.5, 8.1,
+  // without alternatives 3.7, 4.0, 5.0, 5.5; 18 x 50,257 8.6, 7.3, 8.1, 9.0; 35 x 50,257 14.1, 8.5, 8.2, 9.0;
+  // 64 x 50,257 16.5, 9.0, 9.8, 9.0, with the logits out of the L2 22.6, 14.1, 16.1, 18.2; 74 x 50,257
+  // 22.5, 13.9, 8.3, 9.2; 128 x 131,072 over 2 and 1 14.8 and 20.8).
+  // Short rows take half the threads (128 x 4,096: 4.8, with 512 threads 6.1) or a quarter (512 x 1,000:
+  // 5.9, with 256 threads 7.2); long ones that want no alternatives take half of them too once four
+  // blocks an SM do not hold them all (600 x 50,257: 26 and 28, 2,048 x 50,257: 66 and 69; but 512 x
+  // 50,257: 22 and 17).  Rows that fill the SMs have three loads a thread under way, which leaves an SM
+  // the registers for another block (512 x 50,257 with four: 19.8, with three 16.5).
+  const int blocks = vocab <= 24576 ? 1 : rows <= 12 ? 8 : rows <= 64 ? 4 : rows <= 148 ? 2 : 1;
   cudaError_t e;
 #define TL_GO(THREADS, BLOCKS, INFLIGHT)                                                              \
   e = hs::token_logprobs<THREADS, BLOCKS, INFLIGHT>(logprob, rank, top_ids, top_logprobs, top, logits, \
@@ -485,8 +488,9 @@ HS_EXPORT int hs_token_logprobs(float* logprob, int* rank, int* top_ids, float* 
   if (blocks == 8) TL_GO(512, 8, 4);
   else if (blocks == 4) TL_GO(512, 4, 4);
   else if (blocks == 2) TL_GO(512, 2, 4);
+  else if (vocab <= 2048) TL_GO(128, 1, 4);
   else if (vocab <= 8192) TL_GO(256, 1, 4);
-  else if (top == 0 && rows > 148) TL_GO(256, 1, 3);
+  else if (top == 0 && rows > 592) TL_GO(256, 1, 3);
   else TL_GO(512, 1, 3);
 #undef TL_GO
   return e == cudaSuccess ? HS_OK : (int)e;

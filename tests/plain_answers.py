@@ -99,9 +99,11 @@ class PlainAnswerOps(PlainOps):
             empty = bool((x == -math.inf).all())
             m = x.nan_to_num(nan=-math.inf, posinf=math.inf, neginf=-math.inf).max()
             lp = x if empty else (x - m) - torch.log(torch.exp(x - m).sum())
-            order = x.nan_to_num(nan=-math.inf, posinf=math.inf, neginf=-math.inf)
-            # NaN behind -inf: sort by (NaN, -value, index)
-            by = sorted(range(vocab), key=lambda v: (bool(x[v] != x[v]), -float(order[v]), v))
+            # larger first, equal ones by index, NaN behind everything
+            index, nan = torch.arange(vocab), (x != x).cpu()
+            real = index[~nan]
+            by = torch.cat([real[torch.sort(x.cpu()[~nan], descending=True, stable=True).indices],
+                            index[nan]]).tolist()
             t = int(tokens[w])
             if 0 <= t < vocab:
                 logprob[w], rank[w] = lp[t].to(logprob.dtype), by.index(t)

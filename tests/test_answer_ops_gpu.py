@@ -326,7 +326,8 @@ def check_logprobs(ops, logits, tokens, top):
 @pytest.mark.parametrize("rows,vocab,top", [
     (1, 1, 1), (3, 2, 2), (2, 31, 31), (4, 33, 32), (5, 255, 0), (3, 257, 7), (2, 1000, 20),
     (3, 4099, 32), (2, 8193, 1), (1, 50257, 5), (3, 50257, 32), (2, 70001, 20), (300, 130, 20),
-    (700, 67, 3), (150, 8200, 0), (150, 8200, 2)])
+    (700, 67, 3), (150, 8200, 0), (150, 8200, 2),
+    (600, 8200, 0), (20, 24600, 3), (70, 24600, 1)])
 def test_logprobs_follow_the_plain_form(ops, rows, vocab, top):
     gen = torch.Generator().manual_seed(rows * 7 + vocab + top)
     logits = torch.randn(rows, vocab, generator=gen) * 3
