@@ -8,8 +8,9 @@
 //
 // Bound by the bytes, each read and written once: 2,500 pages of 12 entries (1.47 GB one way) take 454 us,
 // 6.5 TB/s, the rate of a plain copy.  A few pages are bound by the launch: 7 half pages of 24
-// entries 3.4 us.  48 pages of 24 entries in float32, half filled, took 25 us as a block a page and
-// entry and 18 as blocks of four rounds of four 16-byte loads a thread (mostly from the L2).
+// entries 3.0 us.  48 pages of 24 entries in float32, half filled, took 25 us as a block a page and
+// entry and 18 in shares with four 16-byte loads a thread under way (mostly from the L2); 20 pages of 13
+// entries of 48 KB filled 9.7 us with shares of 64 KB and 5.5 with shares that give an SM eight blocks.
 #include "common.cuh"
 
 namespace hs {
@@ -64,11 +65,11 @@ cudaError_t copy_pages(void* dst, const void* src, int n, const int* dst_list, c
       list.src[i] = src_list[from + i];
       list.rows[i] = (short)(rows ? rows[from + i] : page_rows);
     }
-    // shares of a page of four rounds of a block's loads or more, two of them at least an SM
+    // shares of a page of up to four rounds of a block's loads, eight of them an SM where the page gives them
     const int row_vecs = (int)(row_bytes / sizeof(V)), page_vecs = tiles * page_rows * row_vecs;
     const int round = PC_INFLIGHT * PC_THREADS;
     int share = 4 * round;
-    while (share > round && (long long)count * entries * ((page_vecs + share - 1) / share) < 2 * 148) share /= 2;
+    while (share > round && (long long)count * entries * ((page_vecs + share - 1) / share) < 8 * 148) share /= 2;
     const int shares = (page_vecs + share - 1) / share;
     if (shares > 65535) return cudaErrorInvalidValue;
     const cudaError_t e = hs_launch(copy_pages_kernel<V, PAIRS>, dim3(count, entries, shares),
