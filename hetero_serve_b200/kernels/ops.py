@@ -216,18 +216,21 @@ def _whole_numbers(given, name, least, most) -> array:
             if given.size and not (least <= int(given.min()) and int(given.max()) <= most):
                 raise OverflowError
             return array("i", given.astype(np.int32).tobytes())
-        out = array("i", given)
-        if len(out) > 64:
+        if len(given) > 64:                      # (packing is the faster way in for a long list)
+            out = array("i", struct.pack(f"{len(given)}i", *given))
             view = np.frombuffer(out, dtype=np.int32)
             low, high = int(view.min()), int(view.max())
-        elif out:
-            low, high = min(out), max(out)
         else:
-            return out
+            out = array("i", given)
+            if not out:
+                return out
+            low, high = min(out), max(out)
         if low < least or high > most:
             raise OverflowError
         return out
-    except TypeError:
+    except (TypeError, struct.error) as exc:
+        if "range" in str(exc) or "format requires" in str(exc):        # struct's overflow
+            raise KernelError(f"copy_pages: {name}: a number lies outside [{least}, {most}]") from None
         raise KernelError(f"copy_pages: {name}: a list of whole numbers wanted") from None
     except OverflowError:
         raise KernelError(f"copy_pages: {name}: a number lies outside [{least}, {most}]") from None
