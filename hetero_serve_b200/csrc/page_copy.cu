@@ -57,6 +57,7 @@ template <typename V, int PAIRS>
 cudaError_t copy_pages(void* dst, const void* src, int n, const int* dst_list, const int* src_list,
                        const int* rows, int entries, int dst_pages, int src_pages, int tiles,
                        int page_rows, int row_bytes, cudaStream_t stream) {
+  const int sms = hs_sm_count();
   for (int from = 0; from < n; from += PAIRS) {
     const int count = n - from < PAIRS ? n - from : PAIRS;
     PageList<PAIRS> list;
@@ -69,7 +70,7 @@ cudaError_t copy_pages(void* dst, const void* src, int n, const int* dst_list, c
     const int row_vecs = (int)(row_bytes / sizeof(V)), page_vecs = tiles * page_rows * row_vecs;
     const int round = PC_INFLIGHT * PC_THREADS;
     int share = 4 * round;
-    while (share > round && (long long)count * entries * ((page_vecs + share - 1) / share) < 8 * 148) share /= 2;
+    while (share > round && (long long)count * entries * ((page_vecs + share - 1) / share) < 8LL * sms) share /= 2;
     const int shares = (page_vecs + share - 1) / share;
     if (shares > 65535) return cudaErrorInvalidValue;
     const cudaError_t e = hs_launch(copy_pages_kernel<V, PAIRS>, dim3(count, entries, shares),

@@ -474,13 +474,15 @@ HS_EXPORT int hs_token_logprobs(float* logprob, int* rank, int* top_ids, float* 
   // turns (us in a graph with 20 alternatives, over 8, 4, 2 and 1 blocks: 1 x 50,257 7.1, 6.7, 7.5, 8.1,
   // without alternatives 3.7, 4.0, 5.0, 5.5; 18 x 50,257 8.6, 7.3, 8.1, 9.0; 35 x 50,257 14.1, 8.5, 8.2, 9.0;
   // 64 x 50,257 16.5, 9.0, 9.8, 9.0, with the logits out of the L2 22.6, 14.1, 16.1, 18.2; 74 x 50,257
-  // 22.5, 13.9, 8.3, 9.2; 128 x 131,072 over 2 and 1 14.8 and 20.8).
+  // 22.5, 13.9, 8.3, 9.2; 128 x 131,072 over 2 and 1 14.8 and 20.8).  Rows up to 24,576 long gain nothing
+  // (32 x 16,384 over one block 5.6, over two 6.6).
   // Short rows take half the threads (128 x 4,096: 4.8, with 512 threads 6.1) or a quarter (512 x 1,000:
   // 5.9, with 256 threads 7.2); long ones that want no alternatives take half of them too once four
   // blocks an SM do not hold them all (600 x 50,257: 26 and 28, 2,048 x 50,257: 66 and 69; but 512 x
   // 50,257: 22 and 17).  Rows that fill the SMs have three loads a thread under way, which leaves an SM
   // the registers for another block (512 x 50,257 with four: 19.8, with three 16.5).
-  const int blocks = vocab <= 24576 ? 1 : rows <= 12 ? 8 : rows <= 64 ? 4 : rows <= 148 ? 2 : 1;
+  const int sms = hs_sm_count();
+  const int blocks = vocab <= 24576 ? 1 : rows <= 12 ? 8 : rows <= 64 ? 4 : rows <= sms ? 2 : 1;
   cudaError_t e;
 #define TL_GO(THREADS, BLOCKS, INFLIGHT)                                                              \
   e = hs::token_logprobs<THREADS, BLOCKS, INFLIGHT>(logprob, rank, top_ids, top_logprobs, top, logits, \
@@ -490,7 +492,7 @@ HS_EXPORT int hs_token_logprobs(float* logprob, int* rank, int* top_ids, float* 
   else if (blocks == 2) TL_GO(512, 2, 4);
   else if (vocab <= 2048) TL_GO(128, 1, 4);
   else if (vocab <= 8192) TL_GO(256, 1, 4);
-  else if (top == 0 && rows > 592) TL_GO(256, 1, 3);
+  else if (top == 0 && rows > 4 * sms) TL_GO(256, 1, 3);
   else TL_GO(512, 1, 3);
 #undef TL_GO
   return e == cudaSuccess ? HS_OK : (int)e;
