@@ -29,7 +29,7 @@ from ..weights import write_model_dir
 from .loading import TORCH_DTYPES, load_model
 from .metrics import RequestRecord, summarise
 from .scheduler import Request, Scheduler, SequenceState
-from .step import Runner, StepEntry, TokenLogprobs
+from .step import Runner, StepEntry, StepError, TokenLogprobs
 
 _scored = itertools.count()
 
@@ -123,11 +123,20 @@ class LLMEngine:
         """Score given text: the log-probability and rank of every token but the first behind the
         ones before it, with the likeliest ``alternatives`` at its place.  Runs beside live
         requests, in portions of the engine's token budget, and needs a state slot and pages for
-        the text meanwhile (:class:`OutOfPages` otherwise)."""
+        the text meanwhile (:class:`OutOfPages` otherwise).  Text with a token outside the
+        vocabulary, or longer than the model, is refused (:class:`StepError`)."""
         runner, text = self.runner, [int(t) for t in token_ids]
-        most = min(MAX_ALTERNATIVES, self.model.spec.vocab_size)
+        vocab = self.model.spec.vocab_size
+        most = min(MAX_ALTERNATIVES, vocab)
         if not 0 <= alternatives <= most:
             raise ValueError(f"{alternatives} alternatives: between 0 and {most}")
+        # Steps take FROM_DEVICE in a portion's first place, and never see the last token.
+        bad = [t for t in text if not 0 <= t < vocab]
+        if bad:
+            raise StepError(f"token id {bad[0]} is outside [0, {vocab})")
+        if len(text) - 1 > runner.max_positions:
+            raise StepError(f"{len(text)} tokens to score: the model has "
+                            f"{runner.max_positions} positions, and the last token needs none")
         name, out = ("score", next(_scored)), []
         with runner._on_device():
             runner.open(name)
@@ -149,6 +158,7 @@ class LLMEngine:
         lps = torch.empty(n, alternatives, device=dev)
         self.runner.ops.token_logprobs(logprob, rank, logits, given,
                                        *((ids, lps) if alternatives else ()))
+        self.runner.check_status()
         return [TokenLogprobs(lp, r, list(zip(i, p))) for lp, r, i, p in
                 zip(logprob.tolist(), rank.tolist(), ids.tolist(), lps.tolist())]
 
