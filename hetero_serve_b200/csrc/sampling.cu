@@ -8,6 +8,9 @@
 // worker.py:647,694) a sampled token does not depend on how requests were batched.  The token
 // is the first, in index order, whose cumulative unnormalised probability exceeds u * total.
 // Ties in argmax and at the top-k threshold go to the lower index.  All arithmetic is float32.
+// A token of weight zero (ruled out: its logit is -inf) is never taken: the threads' sums are joined
+// in another order than each adds its own, so one range may end at or below a target that the next
+// one already begins above, and what stands first there need not weigh anything.
 #include "common.cuh"
 
 namespace hs {
@@ -237,8 +240,10 @@ sample_kernel(int* __restrict__ out, const float* __restrict__ logits,
       int chunk_kept;
       block_scan(cf, dummy, chunk_total, chunk_kept);
       if (pass == 1) {
-        if (kept && run + cf > target) atomicMin(&found, i);
-        if (kept) last_kept = i;
+        if (kept && e != 0.f) {
+          if (run + cf > target) atomicMin(&found, i);
+          last_kept = i;
+        }
         __syncthreads();
         if (found != 0x7fffffff) break;
       }
@@ -248,7 +253,7 @@ sample_kernel(int* __restrict__ out, const float* __restrict__ logits,
   }
   __syncthreads();
   if (found == 0x7fffffff) {
-    // u * total rounded up to the total itself: the last kept token
+    // u * total is no less than the last range's end: the last token with a weight
     __shared__ int lastk;
     if (threadIdx.x == 0) lastk = 0;
     __syncthreads();
@@ -526,7 +531,7 @@ sample_smem_kernel(int* __restrict__ out, const float* __restrict__ logits,
   float run = before;
   for (int i = any ? lo : hi; i < hi; ++i) {
     const float e = s_row[i];
-    if (e >= 0.f) {
+    if (e > 0.f) {
       run += e;
       if (cand == 0x7fffffff && run > target) cand = i;
       last_kept = i;
@@ -536,7 +541,7 @@ sample_smem_kernel(int* __restrict__ out, const float* __restrict__ logits,
   if (last_kept >= 0) atomicMax(&s_last, last_kept);
   __syncthreads();
   if (threadIdx.x == 0) {
-    // u * total rounded up to the total itself: the last kept token
+    // u * total is no less than the last range's end: the last token with a weight
     const int tok = s_found != 0x7fffffff ? s_found : s_last;
     out[rowi] = tok;
     if (fb >= 0) feedback[fb] = tok;
@@ -927,7 +932,7 @@ sample_cluster_kernel(int* __restrict__ out, const float* __restrict__ logits,
     int cand = 0x7fffffff, last_kept = -1;
     for (int i = any ? lo : hi; i < hi; ++i) {
       const float e = s_row[i];
-      if (e >= 0.f) {
+      if (e > 0.f) {
         run += e;
         if (cand == 0x7fffffff && run > target) cand = from + i;
         last_kept = from + i;
@@ -948,7 +953,7 @@ sample_cluster_kernel(int* __restrict__ out, const float* __restrict__ logits,
       found = min(found, s_v[b]);
       last = max(last, s_i[b]);
     }
-    // u * total rounded up to the total itself: the last kept token
+    // u * total is no less than the last range's end: the last token with a weight
     const int tok = found != 0x7fffffff ? found : last;
     out[rowi] = tok;
     if (fb >= 0) feedback[fb] = tok;
