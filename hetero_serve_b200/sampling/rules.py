@@ -22,9 +22,16 @@ from typing import Mapping, Sequence
 import numpy as np
 
 
+# The largest number a rule may hold.  Steps hold them in 32 bits: up to here a finite logit stays
+# finite under any of them, and so does its quotient by a temperature (1e8 * 1e20 + 1e7 * 1e20, for
+# the largest logits and counts there are, is ten decades below the largest number of 32 bits).
+LARGEST = 1e20
+
+
 @dataclass(frozen=True, eq=False)
 class LogitRules:
-    """The numbers of a request's rules; ValueError for numbers no request can mean."""
+    """The numbers of a request's rules; ValueError for numbers no request can mean (beyond
+    ``LARGEST``; a finite bias below ``-LARGEST`` counts as that)."""
 
     repetition: float = 1.0
     presence: float = 0.0
@@ -35,19 +42,21 @@ class LogitRules:
     bias_values: np.ndarray = field(init=False, repr=False)
 
     def __post_init__(self):
-        if not (math.isfinite(self.repetition) and self.repetition > 0):
-            raise ValueError(f"repetition penalty {self.repetition} is not a positive number")
+        if not 1 / LARGEST <= self.repetition <= LARGEST:
+            raise ValueError(f"repetition penalty {self.repetition}: between {1 / LARGEST} and "
+                             f"{LARGEST}")
         for name in ("presence", "frequency"):
-            if not math.isfinite(getattr(self, name)):
-                raise ValueError(f"{name} penalty {getattr(self, name)} is not a finite number")
+            if not abs(getattr(self, name)) <= LARGEST:
+                raise ValueError(f"{name} penalty {getattr(self, name)}: at most {LARGEST} either way")
         for token, value in self.bias.items():
             if isinstance(token, bool) or not isinstance(token, (int, np.integer)) \
                     or not 0 <= token < 2 ** 31:
                 raise ValueError(f"bias of {token!r}, which is no token id")
-            if math.isnan(value) or value == math.inf:
-                raise ValueError(f"bias {value} of token {token}: neither a number nor -inf")
+            if not value <= LARGEST:
+                raise ValueError(f"bias {value} of token {token}: -inf, or a number up to {LARGEST}")
+        values = (v if v == -math.inf else max(v, -LARGEST) for v in self.bias.values())
         for name, kind, of in (("bias_ids", np.int32, self.bias.keys()),
-                               ("bias_values", np.float32, self.bias.values())):
+                               ("bias_values", np.float32, values)):
             object.__setattr__(self, name, np.fromiter(of, dtype=kind, count=len(self.bias)))
 
     @property

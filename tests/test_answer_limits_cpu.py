@@ -1,11 +1,16 @@
 """What may not disturb other requests, without a GPU: bad text to score, numbers out of range, grammars
 that fail, queues, names, refused copies.  The engine over the plain twins of the kernels."""
 
+import math
+
+import numpy as np
 import pytest
 
 from plain_answers import PlainAnswerOps
 from test_answers_cpu import engine
-from hetero_serve_b200 import Request
+from test_scheduler import make, prompt
+from hetero_serve_b200 import LogitRules, Request
+from hetero_serve_b200.engine.scheduler import RequestRefused
 from hetero_serve_b200.engine.step import StepError
 
 
@@ -63,3 +68,51 @@ def test_a_text_longer_than_the_model_is_refused_before_anything_runs(tiny_model
     with pytest.raises(StepError):
         eng.score(tiny.tokens(130, 1))
     assert eng.runner.steps_run == ran and eng.runner.manager.live() == []
+
+
+# -- numbers that 32 bits do not hold -----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("bad", [
+    dict(repetition_penalty=1e-50), dict(repetition_penalty=1e-30), dict(repetition_penalty=1e30),
+    dict(repetition_penalty=1e300), dict(presence_penalty=1e300), dict(presence_penalty=-1e39),
+    dict(presence_penalty=1e30), dict(frequency_penalty=1e300), dict(frequency_penalty=-1e30),
+    dict(logit_bias={3: 1e39}), dict(logit_bias={3: 1e300}), dict(logit_bias={3: 1e30}),
+    dict(logit_bias={3: 3.4e38})])
+def test_numbers_that_leave_no_finite_logit_are_refused(bad, recwarn):
+    sch, _fake, _mgr = make()
+    with pytest.raises(RequestRefused):
+        sch.add(Request(prompt(5), **bad))
+    assert not sch.has_work() and not recwarn.list
+
+
+def test_numbers_at_the_edges_keep_logits_finite(recwarn):
+    """The largest numbers that are taken, over the largest logits and counts there are: finite in 32
+    bits, and still finite divided by a temperature of 1e-6."""
+    most = 1e20
+    low, high = LogitRules(1 / most, -most, -most, {3: most}), LogitRules(most, most, most, {3: -most})
+    for rules in (low, high):
+        for x in (1e8, -1e8, 0.0):
+            y = x / rules.repetition if x > 0 else x * rules.repetition
+            y += rules.bias_values[0] - rules.frequency * 1e7 - rules.presence
+            assert math.isfinite(np.float32(y)) and math.isfinite(np.float32(y / 1e-6))
+    lowest = float(np.finfo(np.float32).min)
+    rules = LogitRules(bias={0: lowest, 1: -1e300, 2: -math.inf, 5: -1e10, 9: 1e-50, 10: 0.1})
+    # finite: not ruled out, and far below every logit
+    assert rules.bias_values.tolist() == [np.float32(-1e20), np.float32(-1e20), -math.inf,
+                                          np.float32(-1e10), 0.0, np.float32(0.1)]
+    assert rules.ruled_out == [2] and not recwarn.list
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.5, 1.0])
+def test_finite_biases_as_low_as_they_go_leave_the_rest(tiny_models, temperature):
+    """Two tokens that a grammar allows, both biased to the type's lowest value: one of them is drawn."""
+    tiny = tiny_models["tiny_b"]
+    lowest = float(np.finfo(np.float32).min)
+
+    class Two:
+        def allowed(self, output):
+            return [4, 9]
+    seq = engine(tiny).submit(Request(tiny.tokens(9, 1), 6, temperature, grammar=Two(),
+                                      logit_bias={4: lowest, 9: lowest}))
+    assert len(seq.output_ids) == 6 and set(seq.output_ids) <= {4, 9}
