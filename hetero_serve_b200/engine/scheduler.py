@@ -412,8 +412,8 @@ class Scheduler:
             if grammar is None or not p.samples:
                 continue
             words = mask_words(grammar.allowed(tuple(p.seq.output_ids)), self.vocab_size)
-            if words is not None and p.seq.rules is not None and len(p.seq.rules.ruled_out):
-                words &= ~mask_words(p.seq.rules.ruled_out, self.vocab_size)
+            if words is not None and p.seq.rules is not None:
+                words = p.seq.rules.leave(words, self.vocab_size)
             if words is not None and not words.any():
                 p.seq.finish_reason = "grammar"
                 self._finish(p.seq, self.clock())

@@ -807,8 +807,10 @@ class Runner:
                     raise StepError(f"request {e.req_id!r}: its mask is not "
                                     f"{history_words(vocab)} int32 words")
                 tail = (1 << (vocab % 32)) - 1 if vocab % 32 else -1
+                if r is not None:
+                    a = r.leave(a, vocab)
                 if not (a[:-1].any() or int(a[-1]) & tail):
-                    raise StepError(f"request {e.req_id!r}: its mask allows no token")
+                    raise StepError(f"request {e.req_id!r}: its mask and biases allow no token")
                 rules = masks = True
             if e.logprobs is not None:
                 if not 0 <= e.logprobs <= min(MAX_ALTERNATIVES, vocab):

@@ -40,6 +40,7 @@ class LogitRules:
     # the biases as arrays, as a step packs them
     bias_ids: np.ndarray = field(init=False, repr=False)
     bias_values: np.ndarray = field(init=False, repr=False)
+    _ruled_words: np.ndarray | None = field(init=False, repr=False, default=None)
 
     def __post_init__(self):
         if not 1 / LARGEST <= self.repetition <= LARGEST:
@@ -64,6 +65,14 @@ class LogitRules:
         """The tokens whose bias is -inf."""
         return self.bias_ids[np.isneginf(self.bias_values)].tolist()
 
+    def leave(self, words: np.ndarray, vocab: int) -> np.ndarray:
+        """A packed mask without the tokens whose bias is -inf."""
+        out = self._ruled_words                    # packed once: steps ask for every row
+        if out is None or len(out) != len(words):
+            out = mask_words(self.ruled_out, vocab)
+            object.__setattr__(self, "_ruled_words", out)
+        return words & ~out
+
     @property
     def penalises(self) -> bool:
         """Whether the record of the request's tokens is needed."""
@@ -74,9 +83,14 @@ class LogitRules:
         return not self.penalises and not len(self.bias_ids)
 
     def check(self, vocab: int | None = None) -> None:
-        """ValueError for a bias of a token the vocabulary does not have."""
-        if vocab is not None and len(self.bias_ids) and int(self.bias_ids.max()) >= vocab:
+        """ValueError for a bias of a token the vocabulary does not have, and for biases that rule
+        all of it out."""
+        if vocab is None or not len(self.bias_ids):
+            return
+        if int(self.bias_ids.max()) >= vocab:
             raise ValueError(f"bias of token {int(self.bias_ids.max())}: the vocabulary has {vocab}")
+        if len(self.bias_ids) >= vocab and len(self.ruled_out) >= vocab:
+            raise ValueError("the biases leave no token")
 
 
 def mask_words(allowed, vocab: int) -> np.ndarray | None:

@@ -9,9 +9,10 @@ import pytest
 from plain_answers import PlainAnswerOps
 from test_answers_cpu import engine
 from test_scheduler import make, prompt
-from hetero_serve_b200 import LogitRules, Request
+from hetero_serve_b200 import LogitRules, Request, StepEntry
 from hetero_serve_b200.engine.scheduler import RequestRefused
 from hetero_serve_b200.engine.step import StepError
+from hetero_serve_b200.sampling import mask_words
 
 
 class ReportingOps(PlainAnswerOps):
@@ -116,3 +117,37 @@ def test_finite_biases_as_low_as_they_go_leave_the_rest(tiny_models, temperature
     seq = engine(tiny).submit(Request(tiny.tokens(9, 1), 6, temperature, grammar=Two(),
                                       logit_bias={4: lowest, 9: lowest}))
     assert len(seq.output_ids) == 6 and set(seq.output_ids) <= {4, 9}
+
+
+# -- rules that leave no token -------------------------------------------------------------------------
+
+
+def test_biases_that_rule_everything_out_are_refused(tiny_models):
+    sch, _fake, _mgr = make()                                     # 97 tokens
+    everything = {t: -math.inf for t in range(97)}
+    with pytest.raises(RequestRefused, match="no token"):
+        sch.add(Request(prompt(5), logit_bias=everything))
+    sch.add(Request(prompt(5), logit_bias={**everything, 96: -1e30}))
+    tiny = tiny_models["tiny_a"]                                  # 512 tokens, 16 words
+    rn = engine(tiny).runner
+    none = LogitRules(bias={t: -math.inf for t in range(512)})
+    even = LogitRules(bias={t: -math.inf for t in range(0, 512, 2)})
+    odd_mask = np.full(16, np.uint32(0xAAAAAAAA)).view(np.int32)
+    for temperature in (0.0, 0.9):
+        for kw in (dict(rules=none), dict(rules=none, allowed=odd_mask), dict(rules=even, allowed=~odd_mask)):
+            with pytest.raises(StepError, match="no token"):
+                rn.step([StepEntry("a", [1, 2], want=[1], temperature=temperature, **kw)], sample=True)
+        assert rn.manager.live() == []
+        res = rn.step([StepEntry("a", [1, 2], want=[1], temperature=temperature, rules=even,
+                                 allowed=odd_mask)], sample=True)
+        assert res.tokens_host()[0] % 2 == 1
+        rn.close("a")
+
+
+def test_masks_without_the_ruled_out_of_any_vocabulary():
+    rules = LogitRules(bias={1: -math.inf, 33: -math.inf, 5: -2.0})
+    for vocab in (40, 97, 40, 64):
+        every = mask_words(range(vocab), vocab)
+        assert np.array_equal(rules.leave(every, vocab),
+                              mask_words([t for t in range(vocab) if t not in (1, 33)], vocab))
+        assert np.array_equal(every, mask_words(range(vocab), vocab))          # the caller's own stays
