@@ -23,6 +23,7 @@ from typing import Sequence
 
 import torch
 
+from ..cache import OutOfPages
 from ..config import EngineConfig, preset
 from ..kernels.ops import MAX_ALTERNATIVES
 from ..weights import write_model_dir
@@ -165,8 +166,13 @@ class LLMEngine:
     def resize_cache(self, num_blocks: int) -> None:
         """Make the cache smaller or larger while requests live: their pages move to the lowest
         numbers of pools of the new size, published prefixes as far as they fit.  Raises
-        :class:`OutOfPages`, with nothing changed, where the live requests' pages do not fit.
-        The longest request the engine takes stays what it was."""
+        :class:`OutOfPages`, with nothing changed, where the live requests' pages do not fit, or a
+        smaller pool would not hold a request that waits.  The longest request the engine takes
+        stays what it was."""
+        for pool, n, promised in zip(self.runner.manager.pools, self.runner.pool_sizes(num_blocks),
+                                     self.scheduler.pages_promised()):
+            if n < min(promised, pool.num_pages):
+                raise OutOfPages(f"a waiting request needs {promised} pages: they do not fit {n}")
         self.runner.resize_cache(num_blocks)
         self.config = replace(self.config, num_blocks=num_blocks)
 

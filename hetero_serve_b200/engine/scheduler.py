@@ -254,6 +254,19 @@ class Scheduler:
     def has_work(self) -> bool:
         return bool(self.waiting or self.active or self._inflight is not None)
 
+    def pages_promised(self) -> list[int]:
+        """Per group the pages that the longest request without a token of its own (or, preempted,
+        without pages) needs: smaller pools would never admit what :meth:`add` took."""
+        promised = [0] * len(self.manager.pools)
+        for seq in [*self.waiting, *self.active]:
+            for s in (seq, *seq.to_fork):
+                if s.admitted and (s.output_ids or s.pending):
+                    continue                        # (ends with what it has, should it come to that)
+                n = len(s.ctx) + (not s.output_ids)
+                for gi in range(len(promised)):
+                    promised[gi] = max(promised[gi], self.manager.pages_for(n, gi))
+        return promised
+
     # -- admission --------------------------------------------------------------
     def _admit(self) -> None:
         """Admit from the front of the queue while a state slot and the pages of the whole

@@ -447,6 +447,11 @@ class Runner:
                     view = t.view(1, t.shape[0], 1, 1, 1, -1)
                     self.ops.copy_pages(view, view, [to], [of])
 
+    def pool_sizes(self, num_pages: int) -> list[int]:
+        """Pages of each group's pool where a runner is made with ``num_pages``."""
+        return [-(-num_pages // g.stride) + self.manager.max_requests if g.stride > 1 else num_pages
+                for g in self.manager.groups]
+
     def resize_cache(self, num_pages: int) -> None:
         """Give the page groups pools of the size ``num_pages`` stands for when a runner is made.
         Live requests keep their pages (moved to the lowest numbers of the new pools), published
@@ -454,8 +459,7 @@ class Runner:
         live requests' pages do not fit; the old and new pools exist side by side meanwhile.  The
         longest request the runner takes (``max_positions``) stays what it was."""
         mgr, model = self.manager, self.model
-        sizes = [-(-num_pages // g.stride) + mgr.max_requests if g.stride > 1 else num_pages
-                 for g in mgr.groups]
+        sizes = self.pool_sizes(num_pages)
         for pool, n in zip(mgr.pools, sizes):
             if n <= 0 or pool.num_held() > n:
                 raise OutOfPages(f"{pool.num_held()} pages are held: they do not fit {n}")

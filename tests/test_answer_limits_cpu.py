@@ -9,7 +9,8 @@ import pytest
 from plain_answers import PlainAnswerOps
 from test_answers_cpu import engine
 from test_scheduler import make, prompt
-from hetero_serve_b200 import LogitRules, Request, StepEntry
+from hetero_serve_b200 import EngineConfig, LLMEngine, LogitRules, Request, StepEntry
+from hetero_serve_b200.cache import OutOfPages
 from hetero_serve_b200.engine.scheduler import RequestRefused
 from hetero_serve_b200.engine.step import StepError
 from hetero_serve_b200.sampling import mask_words
@@ -151,3 +152,84 @@ def test_masks_without_the_ruled_out_of_any_vocabulary():
         assert np.array_equal(rules.leave(every, vocab),
                               mask_words([t for t in range(vocab) if t not in (1, 33)], vocab))
         assert np.array_equal(every, mask_words(range(vocab), vocab))          # the caller's own stays
+
+
+# -- a cache of another size under a queue -----------------------------------------------------------
+
+
+def finish(eng, limit=400):
+    for _ in range(limit):
+        if not eng.has_work():
+            return
+        eng.step()
+        eng.runner.manager.check()
+    raise AssertionError("requests are stuck")
+
+
+def test_a_cache_is_not_made_too_small_for_a_queued_request(tiny_models):
+    """Pages of 16: prompts of 60 and 5 tokens wait; what the longer one needs stays."""
+    tiny = tiny_models["tiny_a"]
+    prompts = [tiny.tokens(60, 1), tiny.tokens(5, 2)]
+    want = engine(tiny).generate(prompts, 4, stop_at_eos=False)
+    eng = engine(tiny)
+    seqs = [eng.submit_nowait(Request(p, 4, stop_at_eos=False)) for p in prompts]
+    for size in (3, 2, 1):
+        with pytest.raises(OutOfPages):
+            eng.resize_cache(size)
+        assert eng.config.num_blocks == 24 == eng.runner.manager.pools[0].num_pages
+    eng.resize_cache(4)
+    finish(eng)
+    assert [s.output_ids for s in seqs] == want
+    eng.resize_cache(2)                                       # nobody waits any more
+    assert eng.submit(Request(prompts[1], 4, stop_at_eos=False)).output_ids == want[1]
+    with pytest.raises(RequestRefused):
+        eng.submit(Request(prompts[0], 4))
+
+
+def test_a_cache_is_not_made_too_small_for_answers_still_to_be_forked(tiny_models):
+    """17 tokens, all but the last resident on one page: every answer needs a second one."""
+    tiny = tiny_models["tiny_a"]
+    p = tiny.tokens(17, 1)
+    want = [r.output_ids for r in engine(tiny).submit_samples(Request(p, 4, 0.9, samples=3, stop_at_eos=False))]
+    eng = engine(tiny, max_prefill_tokens=8)
+    seq = eng.submit_nowait(Request(p, 4, 0.9, samples=3, stop_at_eos=False))
+    eng.step()
+    assert eng.runner.manager.pools[0].num_held() == 1
+    with pytest.raises(OutOfPages):
+        eng.resize_cache(1)
+    eng.resize_cache(2)
+    finish(eng)
+    assert [s.output_ids for s in (seq, *seq.siblings)] == want
+
+
+@pytest.mark.parametrize("pipeline", [False, True])
+def test_preempted_requests_count_and_a_larger_cache_is_never_refused(tiny_models, pipeline):
+    tiny = tiny_models["tiny_a"]
+    prompts = [tiny.tokens(30, 70 + i) for i in range(3)]
+    want = engine(tiny).generate(prompts, 30, stop_at_eos=False)
+    eng = engine(tiny, num_blocks=6, prefix_cache=False, pipeline=pipeline)
+    seqs = [eng.submit_nowait(Request(p, 30, stop_at_eos=False)) for p in prompts]
+    while not eng.scheduler.stats.preemptions:
+        eng.step()
+    waits = max(len(s.ctx) for s in eng.scheduler.waiting)
+    held = eng.runner.manager.pools[0].num_held()
+    for size in range(1, 6):
+        if size < max(held, -(-waits // 16)):
+            with pytest.raises(OutOfPages):
+                eng.resize_cache(size)
+    eng.resize_cache(7)
+    finish(eng)
+    assert [s.output_ids for s in seqs] == want
+
+
+def test_another_size_counts_every_group(putelix_cases):
+    """Windows and companion rows beside full groups: every pool keeps what a queued prompt needs."""
+    case = putelix_cases["case_a"]
+    eng = LLMEngine(case.dir, EngineConfig(dtype="float32", num_blocks=40, max_batch=4, device="cpu",
+                                           max_prefill_tokens=16, cuda_graphs=False), ops=PlainAnswerOps())
+    seq = eng.submit_nowait(Request(case.tokens(50, 1), 2, stop_at_eos=False))
+    with pytest.raises(OutOfPages):
+        eng.resize_cache(3)
+    eng.resize_cache(5)
+    finish(eng)
+    assert len(seq.output_ids) == 2
