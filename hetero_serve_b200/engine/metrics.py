@@ -49,6 +49,7 @@ class RequestRecord:
     t_done: float = 0.0
     # scores of the generated tokens (``TokenLogprobs``), where the request asked for them
     scores: list = field(default_factory=list)
+    error: str = ""                # what its grammar failed with (finish_reason "grammar_error")
 
     @property
     def cumulative_logprob(self) -> float:
@@ -80,6 +81,8 @@ class RequestRecord:
             "prefill_tokens_computed", "preemptions", "finish_reason")}
         out.update(ttft=round(self.ttft, 5), tpot=round(self.tpot, 6), e2e=round(self.e2e, 5),
                    cache_hit_rate=round(self.cache_hit_rate, 4), output_ids=list(self.output_ids))
+        if self.error:
+            out["error"] = self.error
         if self.scores:
             out.update(cumulative_logprob=round(self.cumulative_logprob, 5),
                        logprobs=[round(s.logprob, 5) for s in self.scores],
@@ -96,7 +99,8 @@ class RequestRecord:
                    prefill_tokens_computed=seq.prefill_tokens_computed,
                    preemptions=seq.preemptions, finish_reason=seq.finish_reason,
                    output_ids=list(seq.output_ids), t_submit=seq.t_submit, t_admit=seq.t_admit,
-                   t_first_token=seq.t_first_token, t_done=seq.t_done, scores=list(seq.scores))
+                   t_first_token=seq.t_first_token, t_done=seq.t_done, scores=list(seq.scores),
+                   error=seq.error)
 
 
 def summarise(records: list[RequestRecord], wall_s: float) -> dict:

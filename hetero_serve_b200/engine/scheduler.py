@@ -119,6 +119,7 @@ class SequenceState:
     prefill_tokens_computed: int = 0
     preemptions: int = 0
     finish_reason: str = ""
+    error: str = ""                     # what its grammar failed with (finish_reason "grammar_error")
     pending: int = 0                    # tokens sampled for it that the host has not read yet
     rules: LogitRules | None = None     # None: none that change anything
     recorded: bool = False              # its tokens are on the device, for penalties
@@ -418,17 +419,22 @@ class Scheduler:
 
     def _masks(self, planned: list[Planned]) -> dict:
         """What the planned requests' grammars allow next, packed, by request.  A request whose
-        grammar allows nothing any more (that its biases do not rule out) ends here."""
+        grammar allows nothing any more (that its biases do not rule out) ends here, and so does
+        one whose grammar raises or answers with anything but tokens of the vocabulary."""
         masks = {}
         for p in planned:
             grammar = p.seq.request.grammar
             if grammar is None or not p.samples:
                 continue
-            words = mask_words(grammar.allowed(tuple(p.seq.output_ids)), self.vocab_size)
+            try:
+                words = mask_words(grammar.allowed(tuple(p.seq.output_ids)), self.vocab_size)
+            except Exception as exc:                # the caller's own code: its request alone ends
+                words = None
+                p.seq.error = f"{type(exc).__name__}: {exc}"
             if words is not None and p.seq.rules is not None:
                 words = p.seq.rules.leave(words, self.vocab_size)
-            if words is not None and not words.any():
-                p.seq.finish_reason = "grammar"
+            if p.seq.error or (words is not None and not words.any()):
+                p.seq.finish_reason = "grammar_error" if p.seq.error else "grammar"
                 self._finish(p.seq, self.clock())
                 self._late_done.append(p.seq)
             elif words is not None:

@@ -10,7 +10,8 @@ A *grammar* is any object with ``allowed(output_ids)``: asked before every token
 generated so far, it says which may come next — ``None`` (any), a packed mask (an array of
 ``ceil(vocab / 32)`` 32-bit words, bit v % 32 of word v // 32), an array of truth values over the
 vocabulary, or token ids (anything else that yields whole numbers; 32-bit arrays are masks).  An
-answer that allows nothing ends the request.
+answer that allows nothing ends the request (``finish_reason == "grammar"``), and so does a grammar
+that raises or answers with anything else (``"grammar_error"``; the record's ``error`` says what).
 """
 
 from __future__ import annotations

@@ -233,3 +233,54 @@ def test_another_size_counts_every_group(putelix_cases):
     eng.resize_cache(5)
     finish(eng)
     assert len(seq.output_ids) == 2
+
+
+# -- grammars that fail -----------------------------------------------------------------------------------
+
+
+class Failing:
+    """Allows anything, and fails once ``n`` tokens have been generated."""
+
+    def __init__(self, n, how):
+        self.n, self.how = n, how
+
+    def allowed(self, output):
+        return self.how() if len(output) >= self.n else None
+
+
+def _raise():
+    raise KeyError("no such rule")
+
+
+FAILURES = {"raises": _raise, "outside": lambda: [10 ** 7], "negative": lambda: [-1], "huge": lambda: [2 ** 70],
+            "wide": lambda: np.ones(4000, dtype=bool), "short": lambda: np.zeros(1, dtype=np.int32),
+            "number": lambda: 7, "text": lambda: "ab", "nothing in it": lambda: [None]}
+
+
+@pytest.mark.parametrize("policy", ["prefill_first", "mixed"])
+@pytest.mark.parametrize("pipeline", [False, True])
+@pytest.mark.parametrize("how", FAILURES)
+def test_a_grammar_that_fails_ends_its_own_request(tiny_models, how, pipeline, policy):
+    tiny = tiny_models["tiny_b"]
+    want = engine(tiny).generate([tiny.tokens(30, 2), tiny.tokens(9, 1)], 8, stop_at_eos=False)
+    eng = engine(tiny, pipeline=pipeline, policy=policy)
+    beside = eng.submit_nowait(Request(tiny.tokens(30, 2), 8, stop_at_eos=False))
+    failing = [eng.submit_nowait(Request(tiny.tokens(9, 1), 8, grammar=Failing(n, FAILURES[how]), samples=1 + n,
+                                         stop_at_eos=False)) for n in (0, 1, 3)]
+    records = []
+    for _ in range(200):
+        if eng.has_work():
+            records += eng.step()
+            eng.runner.manager.check()
+    assert not eng.has_work() and beside.output_ids == want[0]
+    for n, seq in zip((0, 1, 3), failing):
+        for s in (seq, *seq.siblings):
+            assert s.finish_reason == "grammar_error" and s.output_ids == want[1][:n] and s.error
+    if how == "raises":
+        assert "no such rule" in failing[0].error
+    by_name = {r.req_id: r for r in records}
+    assert len(by_name) == 1 + 1 + 2 + 4
+    record = by_name[failing[1].req_id]
+    assert record.error == failing[1].error == record.as_dict()["error"]
+    assert by_name[beside.req_id].error == "" and "error" not in by_name[beside.req_id].as_dict()
+    assert eng.runner.manager.free_slots() == eng.config.live_requests
