@@ -17,6 +17,7 @@ that raises or answers with anything else (``"grammar_error"``; the record's ``e
 from __future__ import annotations
 
 import math
+import operator
 from dataclasses import dataclass, field
 from typing import Mapping, Sequence
 
@@ -94,6 +95,12 @@ class LogitRules:
             raise ValueError("the biases leave no token")
 
 
+def _token(t) -> int:
+    if isinstance(t, (bool, np.bool_)) or str(getattr(t, "dtype", "")) == "torch.bool":
+        raise ValueError("truth values outside an array: which tokens are meant?")
+    return operator.index(t)              # (a fraction, or text, is no token id either)
+
+
 def mask_words(allowed, vocab: int) -> np.ndarray | None:
     """What a grammar's ``allowed`` answered as packed int32 words (None: any token)."""
     if allowed is None:
@@ -113,7 +120,10 @@ def mask_words(allowed, vocab: int) -> np.ndarray | None:
             raise ValueError(f"truth values of shape {allowed.shape} for {vocab} tokens")
         flags[:vocab] = allowed
     else:
-        ids = np.fromiter((int(t) for t in allowed), dtype=np.int64)
+        if isinstance(allowed, np.ndarray) and allowed.ndim == 1 and allowed.dtype.kind in "iu":
+            ids = allowed.astype(np.int64)
+        else:
+            ids = np.fromiter((_token(t) for t in allowed), dtype=np.int64)
         if ids.size and (ids.min() < 0 or ids.max() >= vocab):
             raise ValueError(f"a grammar allows a token outside [0, {vocab})")
         flags[ids] = True

@@ -284,3 +284,16 @@ def test_a_grammar_that_fails_ends_its_own_request(tiny_models, how, pipeline, p
     assert record.error == failing[1].error == record.as_dict()["error"]
     assert by_name[beside.req_id].error == "" and "error" not in by_name[beside.req_id].as_dict()
     assert eng.runner.manager.free_slots() == eng.config.live_requests
+
+
+def test_answers_that_are_no_token_ids_are_refused():
+    """A list or tensor of truth values is no list of the tokens 0 and 1, 1.5 is not token 1."""
+    import torch
+    flags = [t % 3 == 0 for t in range(40)]
+    for bad in (flags, torch.tensor(flags), [1.5], [2.0], np.array([1.0, 3.0]), ["7"], [True], [np.True_]):
+        with pytest.raises((TypeError, ValueError)):
+            mask_words(bad, 40)
+    want = mask_words([3, 39], 40)
+    for good in ((3, 39), {3, 39}, range(3, 40, 36), iter([3, 39]), np.array([3, 39]), np.array([3, 39], np.uint8),
+                 [np.int64(3), np.int32(39)], torch.tensor([3, 39]), {3: "a", 39: "b"}):
+        assert np.array_equal(mask_words(good, 40), want)
