@@ -26,6 +26,7 @@ import torch
 from ..cache import OutOfPages
 from ..config import EngineConfig, preset
 from ..kernels.ops import MAX_ALTERNATIVES
+from ..sampling import is_whole
 from ..weights import write_model_dir
 from .loading import TORCH_DTYPES, load_model
 from .metrics import RequestRecord, summarise
@@ -129,7 +130,7 @@ class LLMEngine:
         runner, text = self.runner, [int(t) for t in token_ids]
         vocab = self.model.spec.vocab_size
         most = min(MAX_ALTERNATIVES, vocab)
-        if not 0 <= alternatives <= most:
+        if not (is_whole(alternatives) and 0 <= alternatives <= most):
             raise ValueError(f"{alternatives} alternatives: between 0 and {most}")
         # Steps take FROM_DEVICE in a portion's first place, and never see the last token.
         bad = [t for t in text if not 0 <= t < vocab]

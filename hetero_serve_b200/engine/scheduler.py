@@ -63,7 +63,7 @@ from typing import Callable, Hashable, Mapping, Sequence
 
 from ..cache import CacheManager, OutOfPages
 from ..kernels.ops import MAX_ALTERNATIVES
-from ..sampling import LogitRules, mask_words
+from ..sampling import LogitRules, is_whole, mask_words
 from .step import FROM_DEVICE, StepEntry
 
 
@@ -233,9 +233,10 @@ class Scheduler:
         if request.grammar is not None and self.vocab_size is None:
             raise RequestRefused("a grammar needs a vocabulary size")
         most = MAX_ALTERNATIVES if self.vocab_size is None else min(MAX_ALTERNATIVES, self.vocab_size)
-        if request.logprobs is not None and not 0 <= request.logprobs <= most:
+        if request.logprobs is not None and not (is_whole(request.logprobs)
+                                                 and 0 <= request.logprobs <= most):
             raise RequestRefused(f"logprobs={request.logprobs}: between 0 and {most} alternatives")
-        if request.samples < 1:
+        if not (is_whole(request.samples) and request.samples >= 1):
             raise RequestRefused(f"samples={request.samples}: at least one answer")
         known = {s.req_id for s in [*self.waiting, *self.active]}
         known |= {s.req_id for q in [*self.waiting, *self.active] for s in q.to_fork}

@@ -37,7 +37,7 @@ import torch
 
 from ..cache import CacheManager, CacheStorage, GroupSpec, OutOfPages
 from ..kernels.ops import MAX_ALTERNATIVES, TokenHistory, history_words, size_class
-from ..sampling import LogitRules
+from ..sampling import LogitRules, is_whole
 
 STATUS_BITS = {1: "a token id outside the vocabulary", 2: "a position outside the table",
                4: "a page number outside the pool", 8: "a kernel pipeline timed out",
@@ -817,7 +817,7 @@ class Runner:
                     raise StepError(f"request {e.req_id!r}: its mask and biases allow no token")
                 rules = masks = True
             if e.logprobs is not None:
-                if not 0 <= e.logprobs <= min(MAX_ALTERNATIVES, vocab):
+                if not (is_whole(e.logprobs) and 0 <= e.logprobs <= min(MAX_ALTERNATIVES, vocab)):
                     raise StepError(f"request {e.req_id!r}: {e.logprobs} alternatives; at most "
                                     f"{min(MAX_ALTERNATIVES, vocab)}")
                 top = max(top or 0, e.logprobs)

@@ -5,6 +5,6 @@ before the draw (``rules.py``: penalties, biases, grammars).
 """
 
 from .rule import philox4x32_10, uniform_for_position
-from .rules import LogitRules, OneOf, mask_words
+from .rules import LogitRules, OneOf, is_whole, mask_words
 
-__all__ = ["LogitRules", "OneOf", "mask_words", "philox4x32_10", "uniform_for_position"]
+__all__ = ["LogitRules", "OneOf", "is_whole", "mask_words", "philox4x32_10", "uniform_for_position"]

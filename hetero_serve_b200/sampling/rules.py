@@ -30,6 +30,11 @@ import numpy as np
 LARGEST = 1e20
 
 
+def is_whole(n) -> bool:
+    """Whether ``n`` is a whole number (a truth value is none)."""
+    return isinstance(n, (int, np.integer)) and not isinstance(n, bool)
+
+
 @dataclass(frozen=True, eq=False)
 class LogitRules:
     """The numbers of a request's rules; ValueError for numbers no request can mean (beyond
@@ -52,8 +57,7 @@ class LogitRules:
             if not abs(getattr(self, name)) <= LARGEST:
                 raise ValueError(f"{name} penalty {getattr(self, name)}: at most {LARGEST} either way")
         for token, value in self.bias.items():
-            if isinstance(token, bool) or not isinstance(token, (int, np.integer)) \
-                    or not 0 <= token < 2 ** 31:
+            if not is_whole(token) or not 0 <= token < 2 ** 31:
                 raise ValueError(f"bias of {token!r}, which is no token id")
             if not value <= LARGEST:
                 raise ValueError(f"bias {value} of token {token}: -inf, or a number up to {LARGEST}")

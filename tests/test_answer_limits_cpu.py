@@ -297,3 +297,28 @@ def test_answers_that_are_no_token_ids_are_refused():
     for good in ((3, 39), {3, 39}, range(3, 40, 36), iter([3, 39]), np.array([3, 39]), np.array([3, 39], np.uint8),
                  [np.int64(3), np.int32(39)], torch.tensor([3, 39]), {3: "a", 39: "b"}):
         assert np.array_equal(mask_words(good, 40), want)
+
+
+@pytest.mark.parametrize("bad", [dict(logprobs=2.5), dict(logprobs=2.0), dict(logprobs="2"), dict(logprobs=True),
+                                 dict(samples=2.5), dict(samples=2.0), dict(samples="2"), dict(samples=None)])
+def test_numbers_of_answers_and_alternatives_are_whole(tiny_models, bad):
+    """2.5 alternatives were taken, and the tokens of the step that brought them were lost."""
+    sch, _fake, _mgr = make()
+    with pytest.raises(RequestRefused):
+        sch.add(Request(prompt(5), **bad))
+    assert not sch.has_work()
+    if "logprobs" in bad:
+        eng = engine(tiny_models["tiny_a"])
+        with pytest.raises(StepError):
+            eng.runner.step([StepEntry("a", [1, 2], want=[1], **bad)], sample=True)
+        with pytest.raises(ValueError):
+            eng.score([1, 2, 3], alternatives=bad["logprobs"])
+        assert eng.runner.manager.live() == []
+
+
+def test_whole_numbers_of_any_kind_are_taken(tiny_models):
+    tiny = tiny_models["tiny_a"]
+    eng = engine(tiny)
+    got = eng.submit_samples(Request(tiny.tokens(5, 1), 3, samples=np.int64(2), logprobs=np.int32(2), seed=np.int64(4)))
+    assert [len(r.scores[0].top) for r in got] == [2, 2]
+    assert len(eng.score([1, 2, 3], alternatives=np.int64(2))[0].top) == 2
