@@ -57,7 +57,7 @@ from __future__ import annotations
 
 import itertools
 import time
-from collections import deque
+from collections import Counter, deque
 from dataclasses import dataclass, field, replace
 from typing import Callable, Hashable, Mapping, Sequence
 
@@ -203,6 +203,7 @@ class Scheduler:
         self._in_phase = True
         self._inflight: tuple[list[Planned], object] | None = None   # launched, tokens unread
         self._late_done: list[SequenceState] = []     # finished while a plan was being made
+        self._names: Counter = Counter()              # of the requests that have not ended
 
     # -- submission -----------------------------------------------------------
     def add(self, request: Request) -> SequenceState:
@@ -238,8 +239,6 @@ class Scheduler:
             raise RequestRefused(f"logprobs={request.logprobs}: between 0 and {most} alternatives")
         if not (is_whole(request.samples) and request.samples >= 1):
             raise RequestRefused(f"samples={request.samples}: at least one answer")
-        known = {s.req_id for s in [*self.waiting, *self.active]}
-        known |= {s.req_id for q in [*self.waiting, *self.active] for s in q.to_fork}
         now = self.clock()
         state = lambda r: SequenceState(request=r, t_submit=now,              # noqa: E731
                                         rules=None if rules.neutral else rules)
@@ -247,8 +246,10 @@ class Scheduler:
         for i in range(1, request.samples):
             seq.siblings.append(state(replace(request, seed=request.seed + i, samples=1,
                                               req_id=f"{request.req_id}#{i}")))
-        if request.samples > 1 and known & {s.req_id for s in [seq, *seq.siblings]}:
+        answers = [seq, *seq.siblings]
+        if len(answers) > 1 and any(s.req_id in self._names for s in answers):
             raise RequestRefused(f"request {request.req_id!r} is known already")
+        self._names.update(s.req_id for s in answers)
         seq.to_fork = list(seq.siblings)
         self.waiting.append(seq)
         return seq
@@ -463,6 +464,7 @@ class Scheduler:
                     # it outgrew the whole pool while generating: end it with what it has
                     self.waiting.popleft()
                     head.state, head.finish_reason = SeqState.DONE, "out_of_pages"
+                    self._ended(head)
                     head.t_done = self.clock()
                     self.finished.append(head)
                     self.stats.finished += 1
@@ -562,12 +564,19 @@ class Scheduler:
     def _finish(self, seq: SequenceState, now: float) -> None:
         seq.state = SeqState.DONE
         seq.t_done = now
+        self._ended(seq)
         # what was generated becomes reusable too (worker.py:720-721)
         self.manager.publish(seq.req_id, seq.ctx[: seq.n_kv])
         self.manager.close(seq.req_id)
         self.active.remove(seq)
         self.finished.append(seq)
         self.stats.finished += 1
+
+    def _ended(self, seq: SequenceState) -> None:
+        """Its name may be taken again."""
+        self._names[seq.req_id] -= 1
+        if self._names[seq.req_id] <= 0:
+            del self._names[seq.req_id]
 
     def abort(self, req_id) -> bool:
         """Drop a request wherever it is; what it holds is given back.  Answers that wait to be
@@ -576,6 +585,7 @@ class Scheduler:
             for other in seq.to_fork:
                 if req_id in (seq.req_id, other.req_id):
                     other.state, other.finish_reason = SeqState.DONE, "aborted"
+                    self._ended(other)
             forked = [o for o in seq.to_fork if o.state != SeqState.DONE]
             if seq.req_id != req_id and len(forked) < len(seq.to_fork):
                 seq.to_fork = forked
@@ -586,11 +596,13 @@ class Scheduler:
                 self.manager.close(req_id)
                 self.active.remove(seq)
                 seq.state, seq.finish_reason = SeqState.DONE, "aborted"
+                self._ended(seq)
                 return True
         for seq in list(self.waiting):
             if seq.req_id == req_id:
                 self.waiting.remove(seq)
                 seq.state, seq.finish_reason = SeqState.DONE, "aborted"
+                self._ended(seq)
                 return True
         return False
 

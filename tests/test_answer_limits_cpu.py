@@ -2,6 +2,7 @@
 that fail, queues, names, refused copies.  The engine over the plain twins of the kernels."""
 
 import math
+from collections import deque
 
 import numpy as np
 import pytest
@@ -322,3 +323,50 @@ def test_whole_numbers_of_any_kind_are_taken(tiny_models):
     got = eng.submit_samples(Request(tiny.tokens(5, 1), 3, samples=np.int64(2), logprobs=np.int32(2), seed=np.int64(4)))
     assert [len(r.scores[0].top) for r in got] == [2, 2]
     assert len(eng.score([1, 2, 3], alternatives=np.int64(2))[0].top) == 2
+
+
+# -- names ---------------------------------------------------------------------------------------------
+
+
+def test_submitting_costs_the_same_however_many_wait():
+    """Counted, not timed: nothing waiting is looked at when a request is added."""
+    class Looked(deque):
+        looks = 0
+
+        def __iter__(self):
+            Looked.looks += 1
+            return super().__iter__()
+    sch, _fake, _mgr = make()
+    sch.waiting = Looked()
+    for i in range(50):
+        sch.add(Request(prompt(5), samples=1 + i % 3))
+    assert len(sch.waiting) == 50 and Looked.looks == 0
+
+
+def test_names_are_known_until_their_requests_end():
+    sch, _fake, mgr = make(num_pages=8, page_size=4, prefix_cache=False)
+    new = lambda name, **kw: Request(prompt(6), req_id=name, **{"max_new_tokens": 4, **kw})   # noqa: E731
+    first = sch.add(new("r", samples=3))
+    for name in ("r", "r#1"):
+        with pytest.raises(RequestRefused, match="known"):
+            sch.add(new(name, samples=2))
+    assert sch.abort("r#2")
+    other = sch.add(new("s"))
+    with pytest.raises(RequestRefused):
+        sch.add(new("s", samples=2))
+    for _ in range(200):
+        if sch.has_work():
+            sch.step()
+    assert first.finish_reason == other.finish_reason == first.siblings[0].finish_reason == "max_new_tokens"
+    sch.add(new("r", samples=3)), sch.add(new("s", samples=2))
+    sch.step()
+    assert sch.abort("r") and sch.abort("s")
+    for name in ("r#1", "r#2", "s#1"):
+        sch.abort(name)
+    assert not sch.has_work() and not sch._names
+    # one that outgrows the pool (eight pages of four) ends, and its name with it
+    grown = sch.add(new("g", max_new_tokens=100))
+    for _ in range(200):
+        if sch.has_work():
+            sch.step()
+    assert grown.finish_reason == "out_of_pages" and not sch._names
