@@ -50,7 +50,8 @@ Several answers to one prompt (``Request.samples``).  The prompt is prefilled on
 last token; then the request is forked (``fork_fn``): its full pages are shared, its last page and
 state copied, and every sample decodes on its own, the last prompt token first, with a seed of its
 own (``seed + i``).  A sample for which no page or slot can be had queues as a request of its own
-at the front, and finds the prompt's pages by prefix reuse.
+at the front, and finds the prompt's pages by prefix reuse.  Sample i is named ``{req_id}#{i}``; of two
+requests of one name the later waits until the earlier has ended.
 """
 
 from __future__ import annotations
@@ -277,7 +278,7 @@ class Scheduler:
         mgr = self.manager
         while self.waiting:
             seq = self.waiting[0]
-            if mgr.free_slots() == 0:
+            if mgr.free_slots() == 0 or seq.req_id in mgr:     # (another of its name: after that)
                 return
             ctx = seq.ctx
             target = seq.prefill_target
@@ -309,8 +310,8 @@ class Scheduler:
         queued: list[SequenceState] = []
         for other in seq.to_fork:
             try:
-                if queued:
-                    raise OutOfPages("an earlier answer waits")
+                if queued or other.req_id in self.manager:
+                    raise OutOfPages("an earlier answer waits, or its name is taken")
                 self.fork_fn(seq.req_id, other.req_id)
             except OutOfPages:
                 queued.append(other)
@@ -471,7 +472,7 @@ class Scheduler:
                     return done + [head]
                 raise RequestRefused(
                     f"request {head.req_id!r} cannot be admitted although nothing else is "
-                    f"running: the pool is too small for it")
+                    f"running: the pool is too small for it, or its name is open elsewhere")
             return done
         entries = []
         for p in planned:

@@ -9,7 +9,7 @@ import pytest
 
 from plain_answers import PlainAnswerOps
 from test_answers_cpu import engine
-from test_scheduler import make, prompt
+from test_scheduler import expected_outputs, make, prompt, run
 from hetero_serve_b200 import EngineConfig, LLMEngine, LogitRules, Request, StepEntry
 from hetero_serve_b200.cache import OutOfPages
 from hetero_serve_b200.engine.scheduler import RequestRefused
@@ -370,3 +370,42 @@ def test_names_are_known_until_their_requests_end():
         if sch.has_work():
             sch.step()
     assert grown.finish_reason == "out_of_pages" and not sch._names
+
+
+@pytest.mark.parametrize("policy", ["prefill_first", "mixed"])
+@pytest.mark.parametrize("before", [True, False])
+def test_a_name_that_an_answer_bears_waits_until_it_is_free(policy, before):
+    """A plain request named as another's second answer, submitted before that is forked or after."""
+    sch, _fake, mgr = make(budget=8, policy=policy)
+    seq = sch.add(Request(prompt(20), max_new_tokens=6, seed=3, samples=3, req_id="r"))
+    if not before:
+        for _ in range(4):
+            sch.step()
+        assert "r#1" in mgr
+    plain = sch.add(Request(prompt(7, 2), max_new_tokens=5, req_id="r#1"))
+    last = sch.add(Request(prompt(9, 4), max_new_tokens=5))
+    run(sch, mgr, limit=200)
+    for i, s in enumerate([seq, *seq.siblings]):
+        assert s.output_ids == expected_outputs(prompt(20), 6, seed=3 + i)
+    assert plain.output_ids == expected_outputs(prompt(7, 2), 5)
+    assert last.output_ids == expected_outputs(prompt(9, 4), 5)
+
+
+def test_an_answer_waits_for_its_name():
+    """The plain request runs when the prompt of the other is resident: the fork queues."""
+    sch, _fake, mgr = make(budget=8)
+    sch.add(Request(prompt(30), max_new_tokens=4, req_id="r", samples=3))
+    plain = sch.add(Request(prompt(3), max_new_tokens=20, req_id="r#1"))
+    sch.waiting.reverse()                                          # it is admitted first
+    seq = sch.waiting[-1]
+    run(sch, mgr, limit=200)
+    assert plain.output_ids == expected_outputs(prompt(3), 20)
+    for i, s in enumerate([seq, *seq.siblings]):
+        assert s.output_ids == expected_outputs(prompt(30), 4, seed=i)
+
+
+def test_two_plain_requests_of_one_name_run_in_turn():
+    sch, _fake, mgr = make()
+    both = [sch.add(Request(prompt(5 + i), max_new_tokens=4, req_id="same")) for i in range(2)]
+    run(sch, mgr, limit=50)
+    assert [s.output_ids for s in both] == [expected_outputs(prompt(5 + i), 4) for i in range(2)]
