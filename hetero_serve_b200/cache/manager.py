@@ -27,6 +27,7 @@ into the shared block, heteroserve/worker/worker.py:401-402).
 from __future__ import annotations
 
 import hashlib
+import itertools
 import struct
 from collections import OrderedDict
 from dataclasses import dataclass, field
@@ -175,28 +176,32 @@ class PagePool:
     def num_held(self) -> int:
         return sum(1 for r in self._ref if r > 0)
 
-    def resize(self, num_pages: int) -> dict[int, int]:
-        """Renumber the pages for a pool of ``num_pages``: held ones, and as many of the published
-        ones nobody holds as fit (the oldest are evicted first), get the lowest numbers in their
-        order.  Returns old number -> new number, or raises :class:`OutOfPages` with nothing
-        changed."""
+    def moves(self, num_pages: int) -> dict[int, int]:
+        """What :meth:`resize` would do, with nothing changed: held pages, and as many of the
+        published ones nobody holds as fit (the oldest go first), get the lowest numbers in their
+        order.  Old number -> new number, or :class:`OutOfPages`."""
         held = [p for p in range(self.num_pages) if self._ref[p] > 0]
         if num_pages <= 0 or len(held) > num_pages:
             raise OutOfPages(f"{len(held)} pages are held: they do not fit {num_pages}")
         drop = max(0, len(held) + len(self._evictable) - num_pages)
-        for _ in range(drop):
+        kept = [self._hash_to_page[h] for h in itertools.islice(self._evictable, drop, None)]
+        return {old: new for new, old in enumerate(sorted(held + kept))}
+
+    def resize(self, num_pages: int) -> dict[int, int]:
+        """Renumber the pages for a pool of ``num_pages``: see :meth:`moves`."""
+        moved = self.moves(num_pages)
+        held = [p for p in range(self.num_pages) if self._ref[p] > 0]
+        while len(held) + len(self._evictable) > num_pages:
             h, _none = self._evictable.popitem(last=False)
             del self._page_to_hash[self._hash_to_page.pop(h)]
             self.evictions += 1
-        stay = sorted(held + [self._hash_to_page[h] for h in self._evictable])
-        moved = {old: new for new, old in enumerate(stay)}
         ref = [0] * num_pages
         for old in held:
             ref[moved[old]] = self._ref[old]
         self._ref = ref
         self._hash_to_page = {h: moved[p] for h, p in self._hash_to_page.items()}
         self._page_to_hash = {p: h for h, p in self._hash_to_page.items()}
-        self._free = list(range(num_pages - 1, len(stay) - 1, -1))
+        self._free = list(range(num_pages - 1, len(moved) - 1, -1))
         self.num_pages = num_pages
         return moved
 

@@ -307,23 +307,23 @@ class Scheduler:
     def _fork_samples(self, seq: SequenceState) -> None:
         """The prompt is resident: start the other answers to it."""
         at = self.active.index(seq) + 1
-        queued: list[SequenceState] = []
-        for other in seq.to_fork:
-            try:
-                if queued or other.req_id in self.manager:
-                    raise OutOfPages("an earlier answer waits, or its name is taken")
-                self.fork_fn(seq.req_id, other.req_id)
-            except OutOfPages:
-                queued.append(other)
-                continue
-            other.admitted, other.state, other.n_kv = True, SeqState.RUNNING, seq.n_kv
-            other.cached_prefix_tokens = seq.n_kv
-            other.t_admit = self.clock()
-            self.stats.tokens_saved_by_cache += seq.n_kv
-            self.active.insert(at, other)
-            at += 1
-        seq.to_fork = []
-        self.waiting.extendleft(reversed(queued))
+        todo, seq.to_fork = deque(seq.to_fork), []
+        try:
+            while todo and todo[0].req_id not in self.manager:
+                other = todo[0]
+                try:
+                    self.fork_fn(seq.req_id, other.req_id)
+                except OutOfPages:
+                    break
+                todo.popleft()
+                other.admitted, other.state, other.n_kv = True, SeqState.RUNNING, seq.n_kv
+                other.cached_prefix_tokens = seq.n_kv
+                other.t_admit = self.clock()
+                self.stats.tokens_saved_by_cache += seq.n_kv
+                self.active.insert(at, other)
+                at += 1
+        finally:
+            self.waiting.extendleft(reversed(todo))     # they queue, whatever kept them
 
     # -- planning ----------------------------------------------------------------
     def plan(self) -> list[Planned]:
@@ -489,6 +489,7 @@ class Scheduler:
         result = self.step_fn(entries)
         for p, entry in zip(planned, entries):
             p.seq.recorded |= entry.history is not None
+        resident: list[SequenceState] = []
         n_dec = sum(1 for p in planned if len(p.tokens) == 1 and p.seq.state == SeqState.RUNNING)
         for p in planned:
             seq = p.seq
@@ -501,7 +502,8 @@ class Scheduler:
                     # publish the finished prompt so that others can share it (worker.py:635-645)
                     self.manager.publish(seq.req_id, seq.ctx[: seq.n_kv])
                     seq.state = SeqState.RUNNING
-                    self._fork_samples(seq)
+                    if seq.to_fork:
+                        resident.append(seq)
             if p.samples:
                 seq.pending += 1
         self.stats.steps += 1
@@ -516,6 +518,12 @@ class Scheduler:
             done.extend(self._read(earlier))
         if not self.pipeline:
             done.extend(self._resolve())
+        try:
+            for seq in resident:
+                self._fork_samples(seq)
+        except BaseException:
+            self._late_done.extend(done)            # (the next call tells of them)
+            raise
         return done
 
     def _resolve(self) -> list[SequenceState]:

@@ -429,23 +429,30 @@ class Runner:
         """Open ``child_id`` as a copy of ``req_id`` as it stands: full pages are shared, the rows
         of a partly filled last page, the mixers' state, the token sampled last and the record
         for penalties are copied on the device, behind what has been launched.  Raises
-        :class:`OutOfPages` with nothing changed."""
+        :class:`OutOfPages`, or what a copy was refused with, with nothing opened."""
         mgr = self.manager
         with self._on_device():
             copies = mgr.fork(req_id, child_id)
-            of, to = mgr.slot(req_id), mgr.slot(child_id)
-            for pool, pairs in zip(self.storage.pools, copies):
-                if pairs:
-                    self.ops.copy_pages(pool, pool, [d for _s, d, _n in pairs],
-                                        [s for s, _d, _n in pairs], [n for _s, _d, n in pairs])
-            rows = list(self.storage.states.values()) + [self.feedback.view(-1, 1).view(torch.float32)]
-            if of in self._recorded:
-                rows += [t.view(torch.float32) for t in self.history.tensors()]
-                self._recorded.add(to)
-            for t in rows:                     # a row a slot: a page of one row
-                if t.numel():                  # (a state may be empty: a convolution of one tap)
-                    view = t.view(1, t.shape[0], 1, 1, 1, -1)
-                    self.ops.copy_pages(view, view, [to], [of])
+            try:
+                self._copy_fork(mgr.slot(req_id), mgr.slot(child_id), copies)
+            except BaseException:
+                mgr.close(child_id)
+                raise
+
+    def _copy_fork(self, of: int, to: int, copies) -> None:
+        for pool, pairs in zip(self.storage.pools, copies):
+            if pairs:
+                self.ops.copy_pages(pool, pool, [d for _s, d, _n in pairs],
+                                    [s for s, _d, _n in pairs], [n for _s, _d, n in pairs])
+        rows = list(self.storage.states.values()) + [self.feedback.view(-1, 1).view(torch.float32)]
+        if of in self._recorded:
+            rows += [t.view(torch.float32) for t in self.history.tensors()]
+        for t in rows:                         # a row a slot: a page of one row
+            if t.numel():                      # (a state may be empty: a convolution of one tap)
+                view = t.view(1, t.shape[0], 1, 1, 1, -1)
+                self.ops.copy_pages(view, view, [to], [of])
+        if of in self._recorded:
+            self._recorded.add(to)
 
     def pool_sizes(self, num_pages: int) -> list[int]:
         """Pages of each group's pool where a runner is made with ``num_pages``."""
@@ -468,13 +475,14 @@ class Runner:
                 torch.cuda.synchronize(self.device)
             new = [torch.zeros((old.shape[0], n, *old.shape[2:]), dtype=old.dtype, device=old.device)
                    for old, n in zip(self.storage.pools, sizes)]
-            self._graphs.clear()               # they point into the old pools
-            moves = mgr.resize(sizes)
-            for gi, moved in enumerate(moves):
+            for to, old, pool, n in zip(new, self.storage.pools, mgr.pools, sizes):
+                moved = pool.moves(n)
                 if moved:
-                    self.ops.copy_pages(new[gi], self.storage.pools[gi], list(moved.values()),
-                                        list(moved))
-                self.storage.pools[gi] = new[gi]
+                    self.ops.copy_pages(to, old, list(moved.values()), list(moved))
+            # nothing is refused from here on
+            mgr.resize(sizes)
+            self._graphs.clear()               # they point into the old pools
+            self.storage.pools[:] = new
             if self.fused is not None:
                 from ..parts.fused import plan_fused_decode
                 self.fused = plan_fused_decode(model, self.ops, self.storage, mgr.page_size)

@@ -13,6 +13,7 @@ from test_scheduler import expected_outputs, make, prompt, run
 from hetero_serve_b200 import EngineConfig, LLMEngine, LogitRules, Request, StepEntry
 from hetero_serve_b200.cache import OutOfPages
 from hetero_serve_b200.engine.scheduler import RequestRefused
+from hetero_serve_b200.kernels import KernelError
 from hetero_serve_b200.engine.step import StepError
 from hetero_serve_b200.sampling import mask_words
 
@@ -409,3 +410,95 @@ def test_two_plain_requests_of_one_name_run_in_turn():
     both = [sch.add(Request(prompt(5 + i), max_new_tokens=4, req_id="same")) for i in range(2)]
     run(sch, mgr, limit=50)
     assert [s.output_ids for s in both] == [expected_outputs(prompt(5 + i), 4) for i in range(2)]
+
+
+# -- copies that are refused ------------------------------------------------------------------------------
+
+
+class RefusingOps(PlainAnswerOps):
+    """Refuses the n-th page copy from now on, as the kernel refuses pages beyond its limits."""
+    refuse = None
+
+    def copy_pages(self, *args, **kw):
+        if self.refuse is not None:
+            self.refuse -= 1
+            if self.refuse < 0:
+                raise KernelError("copy_pages: unsupported")
+        super().copy_pages(*args, **kw)
+
+
+def refusing(case):
+    eng = LLMEngine(case.dir, EngineConfig(dtype="float32", num_blocks=40, max_batch=4, device="cpu",
+                                           max_prefill_tokens=64, cuda_graphs=False), ops=RefusingOps())
+    vocab = eng.model.spec.vocab_size
+    return eng, [(7 * i + 3) % vocab for i in range(37)]
+
+
+@pytest.mark.parametrize("at", [0, 1, 2])
+def test_a_fork_whose_copies_are_refused_leaves_nothing_open(putelix_cases, at):
+    """Several groups of pages and the tokens sampled last: copy 0, 1 or 2 of them is refused."""
+    eng, p = refusing(putelix_cases["case_a"])
+    rn = eng.runner
+    rn.step([StepEntry("a", p, want=[36])], sample=True)
+    free = [pool.num_free for pool in rn.manager.pools]
+    rn.ops.refuse = at
+    with pytest.raises(KernelError):
+        rn.fork("a", "b")
+    assert rn.manager.live() == ["a"] and [pool.num_free for pool in rn.manager.pools] == free
+    rn.manager.check()
+    rn.ops.refuse = None
+    rn.fork("a", "b")
+    res = rn.step([StepEntry(r, [5], want=[0]) for r in "ab"], sample=True)
+    assert res.tokens_host()[0] == res.tokens_host()[1]
+
+
+@pytest.mark.parametrize("at", [0, 1])
+def test_a_resize_whose_copies_are_refused_changes_nothing(putelix_cases, at):
+    case = putelix_cases["case_a"]
+    eng, p = refusing(case)
+    want = eng.generate([p], 12, stop_at_eos=False)[0]
+    seq = eng.submit_nowait(Request(p, 12, stop_at_eos=False))
+    for _ in range(3):
+        eng.step()
+    mgr = eng.runner.manager
+    tables = [list(mgr.table(seq.req_id, gi)) for gi in range(len(mgr.groups))]
+    sizes = [pool.num_pages for pool in mgr.pools]
+    eng.runner.ops.refuse = at
+    with pytest.raises(KernelError):
+        eng.resize_cache(30)
+    assert [pool.num_pages for pool in mgr.pools] == sizes == [t.shape[1] for t in eng.runner.storage.pools]
+    assert [list(mgr.table(seq.req_id, gi)) for gi in range(len(mgr.groups))] == tables
+    assert eng.config.num_blocks == 40
+    mgr.check()
+    eng.runner.ops.refuse = None
+    eng.resize_cache(30)
+    finish(eng)
+    assert seq.output_ids == want
+
+
+@pytest.mark.parametrize("pipeline", [False, True])
+def test_refused_copies_of_a_fork_lose_no_token_and_no_answer(tiny_models, pipeline):
+    """The second of three copies is refused, once, in a step that ends another request: that error
+    comes up, and every answer and record comes all the same."""
+    tiny = tiny_models["tiny_b"]
+    p = tiny.tokens(37, 3)
+    ask = lambda: Request(p, 6, 0.9, seed=5, samples=4, stop_at_eos=False, req_id="r")     # noqa: E731
+    want = [r.output_ids for r in engine(tiny).submit_samples(ask())]
+    eng = engine(tiny, pipeline=pipeline, policy="mixed", max_prefill_tokens=64)
+    eng.runner.ops.__class__ = RefusingOps
+    beside = eng.submit_nowait(Request(tiny.tokens(9, 4), 3, stop_at_eos=False, req_id="beside"))
+    eng.step(), eng.step()
+    seq = eng.submit_nowait(ask())
+    eng.runner.ops.refuse = 3                                # (two copies a fork: the page and the token)
+    records, errors = [], 0
+    for _ in range(200):
+        if eng.has_work():
+            try:
+                records += eng.step()
+            except KernelError:
+                errors += 1
+                eng.runner.ops.refuse = None
+            eng.runner.manager.check()
+    assert errors == 1 and not eng.has_work()
+    assert [s.output_ids for s in (seq, *seq.siblings)] == want and len(beside.output_ids) == 3
+    assert sorted(r.req_id for r in records) == ["beside", "r", "r#1", "r#2", "r#3"]
