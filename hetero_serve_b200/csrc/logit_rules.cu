@@ -251,7 +251,9 @@ history_begin_kernel(int* prompt, int* output, int* counts, int vocab, int words
     if (blockIdx.x == 0 && tid == 0) atomicOr(status, HS_STATUS_BAD_ROW);
     return;
   }
-  const int t0 = max(0, start[k]), t1 = min(n_tokens, start[k + 1]), p1 = start[k] + n_prompt[k];
+  const int t0 = max(0, start[k]), t1 = min(n_tokens, start[k + 1]);
+  // (a prompt may be said to be longer than its tokens are, up to any number)
+  const int p1 = (int)min(max((long long)start[k] + n_prompt[k], 0ll), (long long)n_tokens);
   // of two rows of one slot the last counts
   bool again = false;
   for (int j = k + 1 + tid; j < n_rows; j += LH_THREADS) again |= slots[j] == slot;

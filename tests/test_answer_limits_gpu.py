@@ -6,6 +6,7 @@ import torch
 from test_answers_gpu import engine
 from hetero_serve_b200 import Request
 from hetero_serve_b200.engine.step import StepError
+from hetero_serve_b200.kernels import CudaOps, TokenHistory
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +43,17 @@ def test_finite_biases_as_low_as_they_go_leave_the_rest(tiny_models, temperature
     seq = engine(tiny.dir).submit(Request(tiny.tokens(9, 1), 12, temperature, grammar=Two(),
                                           logit_bias={4: lowest, 9: lowest}))
     assert len(seq.output_ids) == 12 and set(seq.output_ids) <= {4, 9}
+
+
+def test_a_prompt_said_to_be_longer_than_its_tokens():
+    """All of a row's tokens are its prompt's then, up to the largest number; none are below zero."""
+    ops = CudaOps()
+    ops.status.zero_()
+    h = TokenHistory.zeros(5, 100, "cuda")
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")          # noqa: E731
+    most = 2 ** 31 - 1
+    ops.history_begin(h, i32([0, 1, 2, 3, 4]), i32([7, 8, 9, 10, 11, 12]), i32([0, 1, 3, 4, 5, 6]),
+                      i32([most, most, most - 2, -1, -most - 1]))
+    assert [r.nonzero().flatten().tolist() for r in h.counts] == [[], [], [], [11], [12]]
+    assert h.prompt[:, 0].tolist() == [1 << 7, (1 << 8) | (1 << 9), 1 << 10, 0, 0]
+    assert int(ops.status.item()) == 0
