@@ -470,12 +470,21 @@ HS_EXPORT int hs_token_logprobs(float* logprob, int* rank, int* top_ids, float* 
   if (rows > (1 << 27) || vocab > 0x7ffffff0) return HS_ERR_UNSUPPORTED;
   cudaStream_t st = (cudaStream_t)stream;
   // A long row over 8, 4 or 2 blocks of 512 threads, as many as find room at once: two such blocks fit an
-  // SM, and a cluster of 8 or 4 needs its SMs in one group of the chip, so that 35 clusters of 8 take
-  // turns (us in a graph with 20 alternatives, over 8, 4, 2 and 1 blocks: 1 x 50,257 7.1, 6.7, 7.5, 8.1,
-  // without alternatives 3.7, 4.0, 5.0, 5.5; 18 x 50,257 8.6, 7.3, 8.1, 9.0; 35 x 50,257 14.1, 8.5, 8.2, 9.0;
-  // 64 x 50,257 16.5, 9.0, 9.8, 9.0, with the logits out of the L2 22.6, 14.1, 16.1, 18.2; 74 x 50,257
-  // 22.5, 13.9, 8.3, 9.2; 128 x 131,072 over 2 and 1 14.8 and 20.8).  Rows up to 24,576 long gain nothing
-  // (32 x 16,384 over one block 5.6, over two 6.6).
+  // SM, and a cluster of 8 or 4 needs its SMs in one group of the chip, so that 35 clusters of 8, and 74 of
+  // 4, take turns on 148 SMs.  us in a graph over 8, 4, 2 and 1 blocks, rows of 50,257 logits:
+  //   rows   without alternatives     with 20
+  //     1     3.7  4.1  4.8  5.8       7.4  7.2  7.3  8.8
+  //    12     4.2  4.6  5.2  6.1       8.4  7.3  7.7  9.3
+  //    24     4.8  5.0  5.4  6.2       9.1  8.1  8.2  9.4
+  //    35     6.9  5.3  5.3  6.1      14.2  8.7  8.2  9.2
+  //    64     8.6  5.9  6.9  6.3      17.1  9.1  9.8  9.3
+  //    74    10.9  8.2  5.5  6.4      22.3 13.9  8.2  9.7
+  //   148    18.5 12.6  7.4  6.5      37.1 21.0 10.8  9.5
+  // (131,072 logits, 20 alternatives: 12 rows 9.1, 8.6, 10.3, 15.2; 128 rows 34.9, 20.9, 15.0, 21.2).  One rule
+  // by rows for both, which costs up to 1.6 us where they differ: 12 rows with 20 alternatives are faster over 4,
+  // 24 without over 8, 148 over one.  Rows up to 24,576 long go to one block: longer ones gain from the cluster
+  // without alternatives first (1 x 24,577 over 8 3.7, over one 3.9; with 20 alternatives 7.0 and 6.1, 64 rows
+  // over 4 8.2, over one 6.6).
   // Short rows take half the threads (128 x 4,096: 4.8, with 512 threads 6.1) or a quarter (512 x 1,000:
   // 5.9, with 256 threads 7.2); long ones that want no alternatives take half of them too once four
   // blocks an SM do not hold them all (600 x 50,257: 26 and 28, 2,048 x 50,257: 66 and 69; but 512 x

@@ -141,7 +141,8 @@ class TokenHistory:
     """Which tokens the request in each state slot holds, in device memory: what penalties for
     repeated tokens go by.  ``prompt`` and ``output`` are bits over the vocabulary (bit v % 32
     of word v // 32: v stands in the prompt; v has been generated), ``counts`` says how often v
-    has been generated and is read only where its output bit is set."""
+    has been generated: rules read it only where its output bit is set, and ``history_add`` counts
+    on from it, so that it is zero where the bit is not."""
 
     prompt: torch.Tensor          # [slots, words] int32
     output: torch.Tensor          # [slots, words] int32
