@@ -514,16 +514,19 @@ class Scheduler:
         else:
             self.stats.mixed_steps += 1
         earlier, self._inflight = self._inflight, (planned, result)
+        failed = None
+        for seq in resident:
+            try:
+                self._fork_samples(seq)
+            except Exception as exc:                # (raised once nothing can be lost by it)
+                failed = failed or exc
         if earlier is not None:
             done.extend(self._read(earlier))
         if not self.pipeline:
             done.extend(self._resolve())
-        try:
-            for seq in resident:
-                self._fork_samples(seq)
-        except BaseException:
+        if failed is not None:
             self._late_done.extend(done)            # (the next call tells of them)
-            raise
+            raise failed
         return done
 
     def _resolve(self) -> list[SequenceState]:

@@ -502,3 +502,25 @@ def test_refused_copies_of_a_fork_lose_no_token_and_no_answer(tiny_models, pipel
     assert errors == 1 and not eng.has_work()
     assert [s.output_ids for s in (seq, *seq.siblings)] == want and len(beside.output_ids) == 3
     assert sorted(r.req_id for r in records) == ["beside", "r", "r#1", "r#2", "r#3"]
+
+
+def test_answers_are_forked_in_a_step_whose_reading_fails(tiny_models):
+    """A kernel's report comes up in the step that makes a prompt resident: its answers run all the same."""
+    tiny = tiny_models["tiny_b"]
+    p = tiny.tokens(37, 3)
+    ask = lambda: Request(p, 6, 0.9, seed=5, samples=3, stop_at_eos=False, req_id="r")     # noqa: E731
+    want = [r.output_ids for r in engine(tiny).submit_samples(ask())]
+    eng = engine(tiny, pipeline=True, policy="mixed", max_prefill_tokens=20)
+    eng.submit_nowait(Request(tiny.tokens(9, 4), 50, stop_at_eos=False, req_id="beside"))
+    eng.step(), eng.step()
+    seq = eng.submit_nowait(ask())
+    eng.runner.status |= 1
+    eng.step()                                              # the first portion; the report rides along
+    with pytest.raises(StepError):
+        eng.step()                                          # the second; the report is read
+    assert [s.state for s in seq.siblings] == ["running", "running"]
+    eng.scheduler.abort("beside")
+    with pytest.raises(StepError):
+        eng.step()                                          # (it was in flight when the report was read)
+    finish(eng)
+    assert [s.output_ids for s in (seq, *seq.siblings)] == want
