@@ -98,7 +98,7 @@ class Request:
     presence_penalty: float = 0.0
     frequency_penalty: float = 0.0
     logit_bias: Mapping[int, float] | None = None
-    grammar: object | None = None       # ``allowed(output_ids)``; a grammar answers for one request
+    grammar: object | None = None       # ``allowed(output_ids)``, asked with each answer's own tokens
     logprobs: int | None = None         # scores of every token, with this many alternatives
     samples: int = 1                    # answers to the prompt; answer i draws with seed + i
 
