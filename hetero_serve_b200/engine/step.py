@@ -30,7 +30,7 @@ from __future__ import annotations
 import contextlib
 import gc
 from dataclasses import dataclass
-from typing import Hashable, Sequence
+from typing import Hashable, NamedTuple, Sequence
 
 import numpy as np
 import torch
@@ -86,9 +86,9 @@ class TokenLogprobs:
     top: list[tuple[int, float]]
 
 
-@dataclass(frozen=True)
-class StepExtras:
-    """What a step does beside running tokens and sampling; part of what its shape is."""
+class StepExtras(NamedTuple):
+    """What a step does beside running tokens and sampling; part of what its shape is, and so of
+    several keys a step (as a tuple it is hashed without a call into Python)."""
 
     rules: bool = False         # some row has penalties, biases or a mask
     history: bool = False       # ... penalties: the record is read and added to
@@ -98,6 +98,9 @@ class StepExtras:
 
     def score_ints(self, rows: int) -> int:
         return 0 if self.top is None else rows * (2 + 2 * self.top)
+
+
+PLAIN = StepExtras()
 
 
 @dataclass
@@ -175,7 +178,7 @@ class Layout:
     """Offsets of the sections of the packed int32 metadata block for one size class."""
 
     def __init__(self, T: int, R: int, W: int, max_pages: Sequence[int], plan_ints: int,
-                 extras: StepExtras = StepExtras(), vocab: int = 0):
+                 extras: StepExtras = PLAIN, vocab: int = 0):
         self.T, self.R, self.W = T, R, W
         self.extras, self.words = extras, history_words(vocab)
         self.max_pages = tuple(max_pages)
@@ -490,7 +493,7 @@ class Runner:
                 torch.cuda.synchronize(self.device)     # the old pools are free from here on
 
     # -- the step -----------------------------------------------------------------
-    def _layout(self, T, R, W, extras: StepExtras = StepExtras()) -> Layout:
+    def _layout(self, T, R, W, extras: StepExtras = PLAIN) -> Layout:
         key = (T, R, W, extras)
         lay = self._layouts.get(key)
         if lay is None:
@@ -553,7 +556,7 @@ class Runner:
             starts.append(start)
             n_tok += n
             n_want += len(e.want)
-        extras = self._extras(entries) if sample else StepExtras()
+        extras = self._extras(entries) if sample else PLAIN
         # Nothing above changed anything.  Requests the cache does not know are opened here and
         # pages are reserved entry by entry; if one cannot be had, what this step took so far
         # is given back, so that a refused step leaves the cache as it found it.
@@ -784,6 +787,8 @@ class Runner:
     def _extras(self, entries) -> StepExtras:
         """What the entries ask for beside tokens; refuses what cannot be given, before anything
         changes."""
+        if all(e.rules is None and e.allowed is None and e.logprobs is None for e in entries):
+            return PLAIN
         vocab = self.model.spec.vocab_size
         rules = history = masks = False
         biases, top = 0, None
